@@ -49,6 +49,7 @@ class Workspace:
         self._bufs: Dict[tuple, torch.Tensor] = {}
         self._views: Dict[tuple, torch.Tensor] = {}      # the first n rows of a buffer, made once per n (a step asks
         self.version = 0                          # bumped when a buffer is replaced (captured graphs go stale)
+        self.kept: Dict[tuple, tuple] = {}        # what a user of a buffer keeps beside it (its tensor map, say)
 
     def rows(self, tag: str, n: int, width: int, dtype: torch.dtype) -> torch.Tensor:
         vkey = (tag, n, width, dtype)             # for the same few dozen views layer after layer)
@@ -82,6 +83,10 @@ class Workspace:
             buf = (torch.zeros if zero else torch.empty)(max(n, 1024), dtype=dtype, device=self.device)
             self._bufs[key] = buf
         return buf[:n]
+
+    def whole(self, tag: str, dtype: torch.dtype) -> torch.Tensor:
+        """All of a `flat` buffer as it stands; replaced when a request for more replaces it."""
+        return self._bufs[(tag, "flat", dtype)]
 
 
 @dataclass

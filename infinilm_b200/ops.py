@@ -1015,7 +1015,7 @@ def stream_status(device) -> torch.Tensor:
 
 # What a kernel whose bounded wait ran out leaves in its stream's status word: from, to, the kernel's file.
 STATUS_CODES = ((11, 14, "gemm_tc5"), (21, 21, "attn_decode"), (30, 39, "attn_prefill_tc5"), (51, 54, "gemm_mid"), (71, 75, "gemm_f32"),
-                (81, 83, "gemm_narrow_tc5"))
+                (81, 83, "gemm_narrow_tc5"), (91, 91, "attn_decode_quant"))
 
 
 def check_status(device) -> None:
@@ -1818,3 +1818,202 @@ def softcap(y: torch.Tensor, cap: float) -> None:
         raise KernelError("softcap: contiguous float32")
     f = _fn("seqmix", "il_softcap", [_c_void_p, _c_float, _c_ll, _c_void_p])
     _check(f(_ptr(y), cap, y.numel(), _stream()), "softcap")
+
+
+# ---- the 8-bit key/value cache -------------------------------------------------------------------
+# One layer's cache is uint8 [pages, kv_heads, 32 * head_dim + 32], pages of 16 tokens: a record per page and kv head (csrc/kv_quant.cuh has the
+# layout and the rounding). A token's K and V rows of a kv head are codes of `kind` times one power of two each.
+KV_KINDS = {"fp8_e4m3": 0, "int8": 1}
+KV_QUANT_PAGE = 16
+QUANT_HEAD_DIMS = (64, 128, 256)                  # head sizes of the attention kernels over this cache
+
+
+def kv_quant_record(head_dim: int) -> int:
+    """Bytes of one page of one kv head."""
+    return 2 * KV_QUANT_PAGE * head_dim + 2 * KV_QUANT_PAGE
+
+
+def _quant_cache(what: str, cache: torch.Tensor, kind: str, n_kv_heads: int, head_dim: int) -> int:
+    """The kind's number, the cache checked."""
+    k = KV_KINDS.get(kind)
+    if k is None:
+        raise KernelError(f"{what}: the cache's kind is one of {', '.join(KV_KINDS)}, not {kind!r}")
+    if (cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[1] != n_kv_heads or cache.shape[2] != 32 * head_dim + 32
+            or not cache.is_contiguous()):
+        raise KernelError(f"{what}: cache uint8 [pages, kv_heads, 32 * head_dim + 32], contiguous")
+    return k
+
+
+def _on_one_device(what: str, *ts: Optional[torch.Tensor]) -> None:
+    """All on the current device, whose current stream the kernels are launched on."""
+    _need_cuda(*ts)
+    d = _cur_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise KernelError(f"{what}: a tensor on {t.device}; the kernels run on the current device, cuda:{d}")
+
+
+def _descriptors(what: str, *ts: Optional[torch.Tensor]) -> None:
+    for t in ts:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise KernelError(f"{what}: descriptors must be contiguous int32")
+
+
+def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tensor, tok_entry: torch.Tensor, block_table: torch.Tensor,
+                     cache: Optional[torch.Tensor], kind: str, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int,
+                     inv_freq: Optional[torch.Tensor], mscale: float) -> None:
+    """Rotates q and k of the rows of `qkv` [T, (heads + 2 kv_heads) * head_dim], writes q to `q_out` [T, heads * head_dim] (of qkv's dtype;
+    its columns of qkv itself, or memory of its own) and k and v as codes to their slots of the 8-bit cache (None: only q). qkv's columns of k and v are left
+    as they are. Each token's slot is its own: what two rows write to one slot is undefined. A token whose block-table entry is below 0 is not stored.
+    A row of k or v that is not finite is stored as NaN."""
+    T, what = qkv.shape[0], "rope_store_quant"
+    if qkv.dim() != 2 or q_out.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1:
+        raise KernelError(f"{what}: qkv [T, (heads + 2 kv_heads) * head_dim], columns side by side")
+    if tuple(q_out.shape) != (T, n_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+        raise KernelError(f"{what}: q_out [T, heads * head_dim] of qkv's dtype, columns side by side")
+    if T == 0:
+        return
+    if q_out.stride(0) < n_heads * head_dim or qkv.stride(0) < qkv.shape[1]:
+        raise KernelError(f"{what}: rows must not overlap")
+    _descriptors(what, tok_pos, tok_entry, block_table)
+    if tok_pos.numel() != T or tok_entry.numel() != T or block_table.dim() != 2:
+        raise KernelError(f"{what}: tok_pos and tok_entry int32 [T], block_table int32 [entries, width]")
+    if rot_dim and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot_dim // 2 or not inv_freq.is_contiguous()):
+        raise KernelError(f"{what}: inv_freq float32 [rot_dim / 2]")
+    k = _quant_cache(what, cache, kind, n_kv_heads, head_dim) if cache is not None else KV_KINDS.get(kind, -1)
+    _on_one_device(what, qkv, q_out, tok_pos, tok_entry, block_table, cache, inv_freq)
+    f = _fn("kv_quant", "il_rope_store_quant", [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int,
+                                                _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_float, _c_void_p])
+    _check(f(_ptr(qkv), kind_of(qkv.dtype), qkv.stride(0), _ptr(q_out), q_out.stride(0), _ptr(tok_pos), _ptr(tok_entry), _ptr(block_table), block_table.shape[1],
+             _ptr(cache), k, T, n_heads, n_kv_heads, head_dim, rot_dim, _ptr(inv_freq if rot_dim else None), mscale, _stream()), what)
+
+
+def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_kvlen: torch.Tensor, pages: torch.Tensor,
+              table: Optional[torch.Tensor] = None, entry_qstart: Optional[torch.Tensor] = None, window: Optional[int] = None,
+              first_entry: int = 0, nan_in_keys: bool = False) -> None:
+    """Reads requests' pages of an 8-bit cache back as values: page p of entry first_entry + i goes to pages[i * width + p], `pages` being bfloat16 or
+    float32 [entries * width, 2, kv_heads, 16, head_dim], the layout of a cache without codes, and `width` the block table's. Every value is exact in both types.
+    Slots behind an entry's length become zeros, whole pages behind it are left as they are; so are, with `entry_qstart` (int32 [entries + 1]: an entry's new tokens
+    are its last qstart[e + 1] - qstart[e]) and `window`, the pages in front of what the first new token sees. A block-table entry below 0 reads as zeros.
+    `table` (int32 of block_table's shape, or None): receives the block table of `pages` for the entries from first_entry on.
+    `nan_in_keys`: for an attention that reads `pages` - a row of V that is NaN comes back as zeros and its row of K as NaN, so that
+    who does not see the key does not get the NaN either."""
+    what = "kv_unpack"
+    if pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[3] != KV_QUANT_PAGE or not pages.is_contiguous():
+        raise KernelError(f"{what}: pages [entries * width, 2, kv_heads, 16, head_dim], contiguous")
+    n_kv_heads, head_dim = pages.shape[2], pages.shape[4]
+    k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
+    _descriptors(what, block_table, entry_kvlen, table, entry_qstart)
+    if block_table.dim() != 2 or not 0 <= first_entry <= block_table.shape[0] or entry_kvlen.numel() < block_table.shape[0]:
+        raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries], first_entry one of them")
+    n_entries, width = block_table.shape
+    if entry_qstart is not None and entry_qstart.numel() < n_entries + 1:
+        raise KernelError(f"{what}: entry_qstart int32 [entries + 1]")
+    if pages.shape[0] < (n_entries - first_entry) * width or (table is not None and tuple(table.shape) != (n_entries, width)):
+        raise KernelError(f"{what}: room for entries * width pages, table of the block table's shape")
+    _on_one_device(what, cache, block_table, entry_kvlen, pages, table, entry_qstart)
+    f = _fn("kv_quant", "il_kv_unpack", [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                         _c_int, _c_void_p, _c_int, _c_void_p])
+    _check(f(_ptr(cache), k, _ptr(block_table), width, _ptr(entry_kvlen), _ptr(entry_qstart), int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
+             _ptr(pages), kind_of(pages.dtype), _ptr(table), int(nan_in_keys), _stream()), what)
+
+
+_resident_quant = {}
+
+
+def _quant_splits(head_dim: int, base: int, pages: int) -> int:
+    """Splits of the keys for `base` blocks a split: as many as fill two thirds of what the device runs at once, at least four pages a split."""
+    key = (_cur_device(), head_dim)
+    n = _resident_quant.get(key)
+    if n is None:
+        fn = build.load("attn_decode_quant", {"HEAD_DIM": head_dim}).il_attn_decode_quant_resident_blocks
+        fn.argtypes, fn.restype = [], _c_int
+        n = _resident_quant[key] = int(fn())
+        if n <= 0:
+            raise KernelError("attention_decode_quant: the occupancy query failed")
+    return max(1, min(n * 2 // 3 // base, (pages + 3) // 4, 128))
+
+
+def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_kvlen: torch.Tensor,
+                           n_decode: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: Optional[int], max_kvlen: int, ws,
+                           cached_before: bool = False) -> None:
+    """Attention of one new token a request over an 8-bit cache: row i of `q` (bfloat16 [rows, >= heads * head_dim], the queries in its first columns) is entry i's
+    token at position entry_kvlen[i] - 1 and sees the keys up to itself, of the last `window` positions if given (negative: of its run of -window positions).
+    `out` bfloat16 [rows, heads * head_dim]; head_dim 64, 128 or 256. A row that sees no key gets zeros; a block-table entry below 0 is never followed, its keys count as masked.
+    max_kvlen: no entry is longer (what the split over the keys is planned for; a larger bound costs time, not results' correctness).
+    ws: a `Workspace` for the splits' partial sums. cached_before: the caller vouches that lengths, block tables and all pages but the newest token's were written before
+    the kernel in front of this call began; they are then read while that kernel still runs."""
+    what = "attention_decode_quant"
+    if n_decode <= 0:
+        return
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1 or not out.is_contiguous():
+        raise KernelError(f"{what}: bfloat16 q [rows, heads * head_dim] and contiguous out")
+    if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads:
+        raise KernelError(f"{what}: head sizes {QUANT_HEAD_DIMS}, heads a multiple of kv_heads")
+    if q.shape[0] < n_decode or q.shape[1] < n_heads * head_dim or out.dim() != 2 or out.shape[0] < n_decode or out.shape[1] != n_heads * head_dim:
+        raise KernelError(f"{what}: q [>= n_decode rows, >= heads * head_dim], out [>= n_decode rows, heads * head_dim]")
+    k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
+    _descriptors(what, block_table, entry_kvlen)
+    if block_table.dim() != 2 or block_table.shape[0] < n_decode or entry_kvlen.numel() < n_decode:
+        raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries]")
+    _on_one_device(what, q, out, cache, block_table, entry_kvlen)
+    w = int(window or 0)
+    seen = max(1, int(max_kvlen)) if not w else max(1, min(int(max_kvlen), abs(w) + KV_QUANT_PAGE))
+    n_splits = _quant_splits(head_dim, n_decode * n_kv_heads * ((n_heads // n_kv_heads + 15) // 16), (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE)
+    o_part = ml_part = None
+    if n_splits > 1:
+        rows = n_decode * n_heads * n_splits
+        o_part, ml_part = ws.flat("quant_o_part", rows * head_dim, torch.float32), ws.flat("quant_ml_part", rows * 2, torch.float32)
+    f = _fn("attn_decode_quant", "il_attn_decode_quant", [_c_void_p, _c_ll, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                                                          _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p],
+            defines={"HEAD_DIM": head_dim})
+    _check(f(_ptr(q), q.stride(0), _ptr(out), _ptr(cache), k, _ptr(block_table), block_table.shape[1], _ptr(entry_kvlen), n_decode, n_heads, n_kv_heads, head_dim,
+             scale, w, n_splits, _ptr(o_part), _ptr(ml_part), _ptr(stream_status(q.device)), int(cached_before), _stream()), what)
+    if n_splits > 1:
+        count_launches(1)                         # the merge kernel
+
+
+def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Consecutive tokens of a request that one block of `attention_prefill_quant` takes: its tiles are counted by this."""
+    return max(1, prefill_tc5_rows(head_dim) // (n_heads // n_kv_heads))
+
+
+def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype):
+    """A workspace's pages for `kv_unpack` ([n_pages, 2, kv_heads, 16, head_dim]) and, for bfloat16, their tensor map (see `kv_tensor_map`; None where there is none)."""
+    per = 2 * n_kv_heads * KV_QUANT_PAGE * head_dim
+    flat = ws.flat("kv_unpacked", n_pages * per, dtype)
+    whole, kept = ws.whole("kv_unpacked", dtype), ws.kept.get(("kv_unpacked", n_kv_heads, head_dim, dtype))
+    if kept is None or kept[0] is not whole:      # (a buffer that grew is another one)
+        full = whole[:whole.numel() // per * per].view(-1, 2, n_kv_heads, KV_QUANT_PAGE, head_dim)
+        kept = ws.kept[("kv_unpacked", n_kv_heads, head_dim, dtype)] = (whole, kv_tensor_map(full) if dtype == torch.bfloat16 else None)
+    return flat.view(n_pages, 2, n_kv_heads, KV_QUANT_PAGE, head_dim), kept[1]
+
+
+def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_qstart: torch.Tensor,
+                            entry_kvlen: torch.Tensor, first_entry: int, n_entries: int, n_tiles_total: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                            scale: float, window: Optional[int], ws, n_tiles_rule: Optional[int] = None) -> None:
+    """Causal attention of the new tokens of entries [first_entry, n_entries) over an 8-bit cache that holds their keys already: entry e's rows of `q` (bfloat16
+    [T, >= heads * head_dim], contiguous, the queries in the first columns) are qstart[e] .. qstart[e + 1], its last tokens. `out` bfloat16 [T, heads * head_dim]; rows of
+    other entries are left as they are. `window` as in `attention_decode_quant`; head_dim 64, 128 or 256, at most 128 query heads a kv head.
+    n_tiles_total = sum over these entries of ceil(new tokens / prefill_quant_tokens(...)); n_tiles_rule as in `attention_prefill_tc5`. ws: a `Workspace` that holds the requests' pages
+    as bfloat16 meanwhile (entries * block-table width pages of one layer)."""
+    what = "attention_prefill_quant"
+    if n_entries <= first_entry or n_tiles_total <= 0:
+        return
+    if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads or not prefill_tc5_ok(head_dim, n_heads // n_kv_heads, KV_QUANT_PAGE):
+        raise KernelError(f"{what}: head sizes {QUANT_HEAD_DIMS}, heads a multiple of kv_heads and at most 128 of them")
+    if q.dim() != 2 or q.shape[1] < n_heads * head_dim or block_table.dim() != 2 or block_table.shape[0] < n_entries or first_entry < 0:
+        raise KernelError(f"{what}: q [T, >= heads * head_dim], block_table int32 [entries, width]")
+    if entry_qstart.numel() < n_entries + 1 or entry_kvlen.numel() < n_entries:
+        raise KernelError(f"{what}: entry_qstart int32 [entries + 1], entry_kvlen int32 [entries]")
+    _descriptors(what, block_table, entry_qstart, entry_kvlen)
+    _on_one_device(what, q, out, cache, block_table, entry_qstart, entry_kvlen)
+    block_table = block_table[:n_entries]
+    width = block_table.shape[1]
+    pages, kv_map = unpacked_cache(ws, (n_entries - first_entry) * width, n_kv_heads, head_dim, torch.bfloat16)
+    if kv_map is None:
+        raise KernelError(f"{what}: the driver has no tensor map for this cache")
+    table = ws.flat("kv_unpacked_table", n_entries * width, torch.int32).view(n_entries, width)
+    kv_unpack(cache, kind, block_table, entry_kvlen, pages, table, entry_qstart, window, first_entry, nan_in_keys=True)
+    attention_prefill_tc5(q, out, kv_map, table, entry_qstart, entry_kvlen, first_entry, n_entries, n_tiles_total, KV_QUANT_PAGE, n_heads, n_kv_heads, head_dim,
+                          scale, window, n_tiles_rule=n_tiles_rule)
