@@ -1,5 +1,6 @@
 // Decode attention over the 8-bit paged cache (kv_quant.cuh): one query token per request in bfloat16, the query heads of a kv
-// head as the 16 rows of a tensor-core tile, the keys of a request split over blocks and merged by a second kernel.
+// head as one or two column tiles of tensor-core products, all requests' pages dealt out evenly to one wave of blocks, what several blocks
+// made of one head's sums added up by a second kernel.
 //
 //   s_k = scale q.K_k with K_k = c_k 2^e_k,  o = sum_k p_k V_k / sum_k p_k,  p_k = 2^(s_k log2 e - m),  V_k = d_k 2^f_k
 //
@@ -9,15 +10,21 @@
 // where they count, and the denominator adds w_k 2^-f_k in 32 bits. One exponential a score, as without a quantised cache. q goes to halves times a
 // power of two of its row's (its largest magnitude then lies in 2^14 .. 2^15): what a half cannot hold of it is below 2^-39 of that.
 //
-//   grid (splits, kv heads * row tiles, entries), 4 warps a block. A warp walks pages p0 + w, p0 + w + 4, ... of its split; a page's record of
-//   a kv head is one untiled bulk copy into the warp's own ring.
-//   Q.K^T: a product step's 16 columns are four codes of each lane of a group of four, so a lane's 16-byte piece of a key row feeds four steps.
-//   P.V: lane (g, q) of a warp takes columns g head_dim/8 .. of keys 2q, 2q + 1, 8 + 2q, 9 + 2q: the keys that its scores belong to; pairs of
-//   keys are joined byte by byte, and tile t of the product holds column t of every lane's columns.
+//   Products: S^T = K.Q^T and O^T = V^T.P^T, keys and V's columns as the 16 rows of a tile, heads as its 8 columns (NT tiles: one up to eight heads a kv head, two
+//   beyond): with the heads as rows, half of every product, softmax and register would belong to rows that are not there where a kv head has eight heads or fewer.
+//   S^T: a product step's 16 columns of K are four codes of each lane of a group of four, so a lane's 16-byte piece of a key row feeds four steps.
+//   O^T: lane (g, q) of a warp takes columns g head_dim/8 .. of keys 2q, 2q + 1, 8 + 2q, 9 + 2q; pairs of keys are joined byte by byte, and tile t holds columns 2t and
+//   2t + 1 of every lane's columns. P goes from the scores' places to the operand's by a transposing move of 8 x 8 halves.
+//
+//   Work: the pages that request e sees, once for each of its units (a kv head, and of its query heads up to 8 NT), one behind the other over requests and units. Block b
+//   takes pages b S .. (b + 1) S of that row, S = all / blocks: requests of any lengths fill the blocks alike. A stretch of one unit is computed by the block's four warps
+//   (warp w takes pages w, w + 4, ... of it; a page's record of a kv head is one untiled bulk copy into the warp's own ring) and merged
+//   in shared memory. A unit that lies in one block is final there, else its parts go to scratch. Short requests (`whole`): a block a unit, all of them final.
+//   (Parts added up by the block that finishes last, with fences and counts, took 8 us more than blocks that are final; the second kernel takes 2 to 3.)
 //
 // Token t (= entry t) sits at position kvlen - 1 and sees positions max(0, kvlen - window) .. kvlen - 1 (window < 0: runs of -window; 0: all). No
-// key to see: zeros. A block-table entry below 0 is never followed, its keys count as masked. A masked key's codes are replaced, so
-// whatever a page holds behind a request's end does not matter.
+// key to see: zeros. A block-table entry below 0 is never followed, its keys count as masked. A masked key's score is replaced and its codes of V cleared, so
+// what a page holds behind a request's end does not matter.
 #include "kv_quant.cuh"
 
 #ifndef HEAD_DIM
@@ -26,26 +33,43 @@
 static_assert(HEAD_DIM == 64 || HEAD_DIM == 128 || HEAD_DIM == 256, "the 8-bit decode kernel takes head_dim 64, 128 or 256");
 
 constexpr int DQ_HD = HEAD_DIM;
-constexpr int DQ_WARPS = 4;
 constexpr int DQ_REC = kvq_record(HEAD_DIM);
-constexpr int DQ_STAGES = HEAD_DIM > 128 ? 3 : 4;
+constexpr int DQ_STAGES = HEAD_DIM > 128 ? 2 : 3;   // records of a warp's ring: more gain nothing (108, 110 us with three and four)
 constexpr int DQ_KG = HEAD_DIM / 64;              // groups of four product steps of Q.K^T
-constexpr int DQ_NT = HEAD_DIM / 8;               // tiles of eight columns of P.V
+constexpr int DQ_MT = HEAD_DIM / 16;              // tiles of 16 columns of V
 constexpr int DQ_VB = HEAD_DIM / 8 < 16 ? HEAD_DIM / 8 : 16;      // columns a lane takes of a key row at a time
 constexpr int DQ_NVB = HEAD_DIM / 8 / DQ_VB;      // ... and how often
-constexpr int DQ_MAX_SPLITS = 128;
+constexpr int DQ_WARPS = 4;
+// Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 13.7 / 11.0 (fewer parts to add up); one of 512 8.0 / 8.6, of 8,192 9.9 / 10.0.
+constexpr int DQ_LEAST = 8;
 constexpr int DQ_OS = HEAD_DIM + 4;
-constexpr int DQ_PIPE = DQ_WARPS * DQ_STAGES * DQ_REC;
-constexpr int DQ_MERGE = DQ_WARPS * 16 * (DQ_OS + 2) * 4;
-constexpr int DQ_BARS = ((DQ_PIPE > DQ_MERGE ? DQ_PIPE : DQ_MERGE) + 15) / 16 * 16;
-constexpr int DQ_SMEM = DQ_BARS + DQ_WARPS * DQ_STAGES * 8;
+// Shared memory of a block: the warps' rings, over them the merge; the rings' barriers behind.
+__host__ __device__ constexpr int dq_bars(int rows) {
+    const int merge = DQ_WARPS * rows * (DQ_OS + 2) * 4 + rows * 8, pipe = DQ_WARPS * DQ_STAGES * DQ_REC;
+    return ((pipe > merge ? pipe : merge) + 15) / 16 * 16;
+}
+__host__ __device__ constexpr int dq_smem(int rows) { return dq_bars(rows) + DQ_WARPS * DQ_STAGES * 8; }
+// Blocks an SM that the registers are to allow.
+constexpr int dq_per_sm(int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 1 ? 4 : 3) : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
 constexpr float DQ_RAISE = 8.f;                   // the running maximum follows only when a page's is more than this above it (log2 units)
 
 __device__ __forceinline__ void dq_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four codes of a word as two pairs of halves. e4m3: bytes 0 and 1, then 2 and 3, by the conversion instruction (shifts and masks instead, which run on another
+// unit, were slower for K, for V and for both: 112, 112 and 123 us where this takes 108, 64 requests of up to 8,192 tokens, 32 heads on 8 of 128). Whole numbers: bytes 0 and 2, then 1 and 3; 1024 + 128 +
+// code as a half is its bits and a constant's, one subtraction leaves the code.
+template <int KIND>
+__device__ __forceinline__ void dq_halves(uint32_t w, uint32_t& a, uint32_t& b) {
+    if constexpr (KIND == KVQ_E4M3) {
+        a = kvq_low<KIND>(w), b = kvq_high<KIND>(w);
+    } else {
+        asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(a) : "r"((w & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(b) : "r"((w >> 8 & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+    }
 }
 __device__ __forceinline__ bool dq_wait(uint32_t bar, uint32_t parity) {
     for (unsigned spin = 0; spin < DQ_SPIN; ++spin) {
@@ -66,360 +90,574 @@ __device__ __forceinline__ uint32_t dq_pack_half(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(hi), "f"(lo));
     return h;
 }
+__device__ __forceinline__ uint32_t dq_transpose(uint32_t x) {       // of 8 x 8 halves: lane (g, q) has row g, columns 2q and 2q + 1
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t dq_pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// (q, the newest token's slot of the cache, and o_part / ml_part in the merge, are written by the kernel before and read after a wait that is not the
+// Pages that a token at the end of kvlen tokens sees, and the first of them.
+__device__ __forceinline__ int dq_pages(int kvlen, int window, int* first) {
+    *first = il_mask_lo(kvlen - 1, window) / KVQ_PAGE;
+    return kvlen > 0 ? (kvlen - 1) / KVQ_PAGE - *first + 1 : 0;
+}
+// How the pages of all requests are dealt out: pages of all units, pages of a block, and the request that page block * share belongs to, with how many pages lie in front of
+// that request's. Every warp makes it for itself.
+struct DqDeal {
+    int all, share, e, before;
+};
+__device__ __forceinline__ DqDeal dq_deal(const int* entry_kvlen, int n_decode, int window, int units, int n_blocks, int block, int lane) {
+    DqDeal d;
+    int first, n0 = 0;
+    d.all = 0;
+    for (int e0 = 0; e0 < n_decode; e0 += 32) {
+        const int n = e0 + lane < n_decode ? dq_pages(entry_kvlen[e0 + lane], window, &first) : 0;
+        d.all += __reduce_add_sync(0xffffffffu, n);
+        if (e0 == 0) n0 = n;
+    }
+    d.all *= units;
+    d.share = max(DQ_LEAST, (int)(((unsigned)d.all + n_blocks - 1) / (unsigned)n_blocks));
+    d.e = 0, d.before = 0;
+    const long long from = (long long)block * d.share;
+    if (from >= d.all) return d;
+    int seen = 0;
+    for (int e0 = 0; e0 < n_decode; e0 += 32) {
+        const int n = e0 == 0 ? n0 : e0 + lane < n_decode ? dq_pages(entry_kvlen[e0 + lane], window, &first) : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int s = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += s;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, seen + sum * units > (int)from);
+        if (past) {
+            const int l0 = __ffs(past) - 1;
+            d.e = e0 + l0, d.before = seen + __shfl_sync(0xffffffffu, sum - n, l0) * units;
+            break;
+        }
+        seen += __shfl_sync(0xffffffffu, sum, 31) * units;
+    }
+    return d;
+}
+// Where a unit's parts lie: its first block's second place, the others' first (a block holds at most the end of one unit and the start of another).
+__device__ __forceinline__ int dq_place(int b0, int i) { return i == 0 ? 2 * b0 + 1 : 2 * (b0 + i); }
+
+// A row's sums, four columns of it: final to `out`, else as a part.
+__device__ __forceinline__ void dq_write(const float4& acc, float M, float L, __nv_bfloat16* out, float* o_part, float* ml_part, int r, int d) {
+    if (out) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;           // (no key seen: zeros)
+        *reinterpret_cast<uint2*>(out + (size_t)r * DQ_HD + d) = make_uint2(dq_pack_bf16(acc.x * inv, acc.y * inv), dq_pack_bf16(acc.z * inv, acc.w * inv));
+    } else {
+        *reinterpret_cast<float4*>(o_part + r * DQ_HD + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(ml_part + 2 * r) = make_float2(M, L);
+    }
+}
+// (q and the newest token's slot of the cache, and in the second kernel the parts, are written by the kernel before and read after a wait that is not the
 // kernel's first statement: they are not declared __restrict__.)
-template <int KIND>
-__global__ void __launch_bounds__(DQ_WARPS * 32) attn_decode_quant_kernel(
+template <int KIND, int NT>
+__global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quant_kernel(
     const __nv_bfloat16* q, long long q_stride, const unsigned char* cache, const int* __restrict__ block_table, int bt_stride,
-    const int* __restrict__ entry_kvlen, int nh, int nkv, float scale_log2, int window, int n_splits, float* o_part, float* ml_part,
-    __nv_bfloat16* out_direct, int* status, int early) {
+    const int* __restrict__ entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int whole, float* o_part, float* ml_part,
+    __nv_bfloat16* out, int* status, int early) {
     if (!early) il_pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
-    const int split = blockIdx.x, G = nh / nkv, row_tiles = (G + 15) / 16;
-    const int head = blockIdx.y / row_tiles, rt = blockIdx.y - head * row_tiles, e = blockIdx.z;
+    constexpr int ROWS = 8 * NT, BARS = dq_bars(ROWS);
+    const int units = nkv * row_tiles, n_blocks = gridDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lq = lane & 3;
-    const int head0 = head * G + rt * 16, rows_valid = min(16, G - rt * 16);
 
     // early: the caller vouches that lengths, block tables and the pages of earlier tokens do not come from the kernel in front (which writes q and
     // the newest token's slot, in the last page). What depends only on them is then done before waiting for it.
-    const int kvlen = entry_kvlen[e];
-    const int lo = il_mask_lo(kvlen - 1, window);
-    const int first_page = lo / KVQ_PAGE, last_page = kvlen > 0 ? (kvlen - 1) / KVQ_PAGE : first_page - 1;
-    const int per_split = (last_page - first_page + n_splits) / n_splits;       // the request's pages, evenly over the splits
-    const int p0 = first_page + split * per_split, p1 = min(p0 + per_split, last_page + 1);
-    if (p0 >= p1 && (split > 0 || !out_direct)) return;       // no keys here: the merge knows; where there is none the block below writes zeros
+    int from, to, e, before;
+    if (whole) {                                  // one unit
+        int first;
+        e = blockIdx.x / units, before = 0;
+        const int n = dq_pages(entry_kvlen[e], window, &first);
+        from = (blockIdx.x - e * units) * n, to = from + n;
+    } else {
+        const DqDeal d = dq_deal(entry_kvlen, n_decode, window, units, n_blocks, blockIdx.x, lane);
+        e = d.e, before = d.before;
+        from = min((long long)blockIdx.x * d.share, (long long)d.all), to = min((long long)from + d.share, (long long)d.all);
+    }
 
-    const int* bt = block_table + (size_t)e * bt_stride;
-    const unsigned char* recs = cache + (size_t)head * DQ_REC;
-    const size_t page_bytes = (size_t)nkv * DQ_REC;
-    const int n_my = max(0, (p1 - p0 - warp + DQ_WARPS - 1) / DQ_WARPS);
-    // Page ids of this warp's iterations, 32 at a time: lane l holds the id of iteration base + l.
-    int ids_base = 0, my_ids = lane < n_my ? bt[p0 + warp + lane * DQ_WARPS] : 0;
-    unsigned bad = 0;                             // bit (iteration % 32): the page is not there, its keys are masked
     const uint32_t pipe = (uint32_t)__cvta_generic_to_shared(smem) + warp * DQ_STAGES * DQ_REC;
-    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + DQ_BARS + warp * DQ_STAGES * 8;
-    const auto issue = [&](int it) {
-        if (it >= n_my) return;
-        if (it >= ids_base + 32) {
-            ids_base += 32;
-            my_ids = ids_base + lane < n_my ? bt[p0 + warp + (ids_base + lane) * DQ_WARPS] : 0;
-        }
-        const int page = __shfl_sync(0xffffffffu, my_ids, it - ids_base);
-        bad = page < 0 ? bad | 1u << (it & 31) : bad & ~(1u << (it & 31));
-        if (lane == 0) {
-            const uint32_t dst = pipe + (it % DQ_STAGES) * DQ_REC, bar = bars + (it % DQ_STAGES) * 8;
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");      // the record before was read by ordinary loads
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(DQ_REC) : "memory");
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                         ::"r"(dst), "l"(recs + (size_t)max(page, 0) * page_bytes), "r"(DQ_REC), "r"(bar) : "memory");
-        }
-    };
+    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + BARS + warp * DQ_STAGES * 8;
+    const size_t page_bytes = (size_t)nkv * DQ_REC;
     if (lane == 0) {
         for (int s = 0; s < DQ_STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(bars + s * 8));
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncwarp();
-    int issued = 0;
-    if (early) {
-        for (; issued < DQ_STAGES && p0 + warp + issued * DQ_WARPS < last_page; ++issued) issue(issued);
-        il_pdl_wait();
-    }
-    for (; issued < DQ_STAGES; ++issued) issue(issued);
+    int done = 0;                                 // records this warp has been through: the ring's place and parity
+    bool waited = !early, dead = false;
+    for (int at = from, unit = 0; at < to;) {
+        // ---- one stretch: pages p0 .. p1 of unit (e, head, rt), which starts at page `start` of the row
+        int first_page, kvlen = entry_kvlen[e], n_pages = dq_pages(kvlen, window, &first_page);
+        while (at >= before + n_pages * units) {
+            before += n_pages * units;
+            kvlen = entry_kvlen[++e], n_pages = dq_pages(kvlen, window, &first_page);
+        }
+        unit = at == from ? (at - before) / n_pages : at == before ? 0 : unit + 1;
+        const int head = row_tiles == 1 ? unit : unit / row_tiles, rt = unit - head * row_tiles;
+        const int start = before + unit * n_pages, end = min(start + n_pages, to);
+        const int p0 = first_page + at - start, p1 = first_page + end - start, last_page = first_page + n_pages - 1;
+        at = end;
+        const int lo = il_mask_lo(kvlen - 1, window), head0 = head * G + rt * ROWS, rows_valid = min(ROWS, G - rt * ROWS);
+        const int* bt = block_table + (size_t)e * bt_stride;
+        const unsigned char* recs = cache + (size_t)head * DQ_REC;
+        const int n_my = dead ? 0 : max(0, (p1 - p0 - warp + DQ_WARPS - 1) / DQ_WARPS);
+        // q's rows are on their way while the pages' are asked for: head 8 j + lg, of each group of 64 columns the 16 from 16 lq on
+        uint32_t qx[NT][8 * DQ_KG];
+        const auto load_q = [&]() {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int r = 8 * j + lg;
+                const __nv_bfloat16* row = q + (size_t)e * q_stride + (size_t)(head0 + r) * DQ_HD;
+#pragma unroll
+                for (int kg = 0; kg < DQ_KG; ++kg)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint4 w = r < rows_valid ? *reinterpret_cast<const uint4*>(row + 64 * kg + 16 * lq + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+                        qx[j][8 * kg + 4 * c] = w.x, qx[j][8 * kg + 4 * c + 1] = w.y, qx[j][8 * kg + 4 * c + 2] = w.z, qx[j][8 * kg + 4 * c + 3] = w.w;
+                    }
+            }
+        };
+        if (waited) load_q();
+        // Page ids of this warp's iterations, 32 at a time: lane l holds the id of iteration base + l.
+        int ids_base = 0, my_ids = lane < n_my ? bt[p0 + warp + lane * DQ_WARPS] : 0;
+        unsigned bad = 0;                         // bit (iteration % 32): the page is not there, its keys are masked
+        const auto issue = [&](int it) {
+            if (it >= n_my) return;
+            if (it >= ids_base + 32) {
+                ids_base += 32;
+                my_ids = ids_base + lane < n_my ? bt[p0 + warp + (ids_base + lane) * DQ_WARPS] : 0;
+            }
+            const int page = __shfl_sync(0xffffffffu, my_ids, it - ids_base);
+            bad = page < 0 ? bad | 1u << (it & 31) : bad & ~(1u << (it & 31));
+            if (lane == 0) {
+                const int place = (done + it) % DQ_STAGES;
+                const uint32_t dst = pipe + place * DQ_REC, bar = bars + place * 8;
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the place was read (or written by the merge) by ordinary instructions
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(DQ_REC) : "memory");
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                             ::"r"(dst), "l"(recs + (size_t)max(page, 0) * page_bytes), "r"(DQ_REC), "r"(bar) : "memory");
+            }
+        };
+        int issued = 0;
+        if (!waited) {
+            for (; issued < DQ_STAGES && p0 + warp + issued * DQ_WARPS < last_page; ++issued) issue(issued);
+            il_pdl_wait();
+            waited = true;
+            load_q();
+        }
+        for (; issued < DQ_STAGES; ++issued) issue(issued);
 
-    // Q as the products' left operand: rows lg and lg + 8, of each group of 64 columns the 16 from 16 lq on.
-    uint32_t qf[4 * DQ_KG][4];
-    float s_scale[2];                             // what a row's score is multiplied by (its power of two taken back)
+        // Q as the products' right operand
+        uint32_t qf[4 * DQ_KG][NT][2];
+        il_f2 s_scale[NT];                        // what the scores of heads 8 j + 2 lq, + 1 are multiplied by (q's power of two taken back)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = lg + 8 * h;
-        const __nv_bfloat16* row = q + (size_t)e * q_stride + (size_t)(head0 + r) * DQ_HD;
-        uint32_t x[8 * DQ_KG], most = 0u;
+        for (int j = 0; j < NT; ++j) {
+            uint32_t most = 0u;
+            const uint32_t* x = qx[j];
 #pragma unroll
-        for (int kg = 0; kg < DQ_KG; ++kg)
+            for (int c = 0; c < 8 * DQ_KG; ++c) most = max(most, max(x[c] & 0x7fffu, x[c] >> 16 & 0x7fffu));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int ex = max((int)(most >> 7) - 127, -100);
+            const float up = __int_as_float((127 + 14 - ex) << 23), back = scale_log2 * __int_as_float((127 - 14 + ex) << 23);
+            s_scale[j] = il_f2_make(__shfl_sync(0xffffffffu, back, 8 * lq), __shfl_sync(0xffffffffu, back, 8 * lq + 4));
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                x[8 * kg + c] = r < rows_valid ? *reinterpret_cast<const uint32_t*>(row + 64 * kg + 16 * lq + 2 * c) : 0u;
-                most = max(most, max(x[8 * kg + c] & 0x7fffu, x[8 * kg + c] >> 16 & 0x7fffu));
+            for (int i = 0; i < 4 * DQ_KG; ++i) {
+                const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i]), b = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i + 1]);
+                const float x0 = __low2float(a) * up, x1 = __high2float(a) * up, x2 = __low2float(b) * up, x3 = __high2float(b) * up;
+                qf[i][j][0] = KIND == KVQ_E4M3 ? dq_pack_half(x0, x1) : dq_pack_half(x0, x2);          // (in the order in which K's codes come)
+                qf[i][j][1] = KIND == KVQ_E4M3 ? dq_pack_half(x2, x3) : dq_pack_half(x1, x3);
             }
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int ex = max((int)(most >> 7) - 127, -100);
-        const float up = __int_as_float((127 + 14 - ex) << 23);
-        s_scale[h] = scale_log2 * __int_as_float((127 - 14 + ex) << 23);
-#pragma unroll
-        for (int i = 0; i < 4 * DQ_KG; ++i) {
-            const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i]), b = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i + 1]);
-            qf[i][h] = dq_pack_half(__low2float(a) * up, __high2float(a) * up);
-            qf[i][2 + h] = dq_pack_half(__low2float(b) * up, __high2float(b) * up);
         }
-    }
 
-    float o[DQ_NT][4];
+        float o[DQ_MT][NT][4];                    // columns 2 t, 2 t + 1 of lane lg's (elements 0, 1 and 2, 3), heads 8 j + 2 lq, + 1
 #pragma unroll
-    for (int i = 0; i < DQ_NT; ++i)
+        for (int t = 0; t < DQ_MT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int it = 0; it < n_my; ++it) {
-        if (!dq_wait(bars + (it % DQ_STAGES) * 8, (it / DQ_STAGES) & 1)) {
-            if (lane == 0) atomicExch(status, 91);
-            for (int k = it + 1; k < min(it + DQ_STAGES, n_my); ++k) dq_wait(bars + (k % DQ_STAGES) * 8, (k / DQ_STAGES) & 1);
-            break;
-        }
-        const unsigned char* rec = smem + (size_t)(warp * DQ_STAGES + it % DQ_STAGES) * DQ_REC;
-        // ---- scores of the page's 16 keys: s[n] holds keys 8 n + 2 lq, + 1 of rows lg (0, 1) and lg + 8 (2, 3)
-        float s[2][4];
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+                for (int i = 0; i < 4; ++i) o[t][j][i] = 0.f;
+        float m[NT][2];
+        il_f2 l[NT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
-#pragma unroll
-        for (int kg = 0; kg < DQ_KG; ++kg)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int key = 8 * n + lg, piece = (key * (DQ_HD / 16) + 4 * kg + lq) ^ kvq_turn(DQ_HD, false, key);
-                const uint4 w = *reinterpret_cast<const uint4*>(rec + piece * 16);
-                const uint32_t c[4] = {kvq_raw<KIND>(w.x), kvq_raw<KIND>(w.y), kvq_raw<KIND>(w.z), kvq_raw<KIND>(w.w)};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dq_mma(s[n], qf[4 * kg + i], kvq_low<KIND>(c[i]), kvq_high<KIND>(c[i]));
+        for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY, l[j] = il_f2_dup(0.f);
+        for (int it = 0; it < n_my; ++it) {
+            if (!dq_wait(bars + (done + it) % DQ_STAGES * 8, (done + it) / DQ_STAGES & 1)) {
+                if (lane == 0) atomicExch(status, 91);
+                for (int k = it + 1; k < min(it + DQ_STAGES, n_my); ++k) dq_wait(bars + (done + k) % DQ_STAGES * 8, (done + k) / DQ_STAGES & 1);
+                dead = true;
+                break;
             }
-        // ---- exponents of this lane's four keys, softmax in base 2
-        uint32_t ke[2], ve[2];
+            const unsigned char* rec = smem + (size_t)(warp * DQ_STAGES + (done + it) % DQ_STAGES) * DQ_REC;
+            // ---- scores of the page's 16 keys: elements 0, 1 are key lg and heads 8 j + 2 lq, + 1; elements 2, 3 key 8 + lg
+            float s[NT][4], s1[NT][4];            // (two chains of products: one is all latency)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            ke[n] = *reinterpret_cast<const uint16_t*>(rec + 2 * KVQ_PAGE * DQ_HD + 8 * n + 2 * lq);
-            ve[n] = *reinterpret_cast<const uint16_t*>(rec + 2 * KVQ_PAGE * DQ_HD + KVQ_PAGE + 8 * n + 2 * lq);
-        }
-        const int key0 = (p0 + warp + it * DQ_WARPS) * KVQ_PAGE + 2 * lq;
-        const bool gone = (bad >> (it & 31)) & 1;
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};        // a byte a key: 2 lq, 2 lq + 1 of either half of the page
-        float inv_v[2][2];
-        const bool edge = gone || key0 - 2 * lq < lo || key0 - 2 * lq + KVQ_PAGE > kvlen;
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+                for (int i = 0; i < 4; ++i) s[j][i] = s1[j][i] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int kb = ke[n] >> (8 * j) & 255, vb = ve[n] >> (8 * j) & 255, key = key0 + 8 * n + j;
-                const float kp = kvq_power(kb), add = vb == KVQ_NAN ? __int_as_float(0x7fc00000) : (float)(vb - 127);
-                const bool there = !edge || (!gone && key >= lo && key < kvlen);
-                inv_v[n][j] = __int_as_float((254 - vb) << 23);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) s[n][2 * h + j] = there ? fmaf(s[n][2 * h + j], s_scale[h] * kp, add) : -INFINITY;
-                if (!there) seen[n] &= j ? 0x00ff00ffu : 0xff00ff00u, inv_v[n][j] = 0.f;
-            }
-        uint32_t pf[4];
-        float corr[2];
-        bool raise = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const bool up = mx > m[h] + DQ_RAISE;             // also the first keys of a row (m = -inf)
-            const float mn = up ? mx : m[h];
-            corr[h] = up ? dq_ex2(m[h] - mn) : 1.f;           // 0 when nothing was summed yet
-            raise |= up;
-            const float ms = mn == -INFINITY ? 0.f : mn;
-            float w[2][2], rs = 0.f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    w[n][j] = dq_ex2(s[n][2 * h + j] - ms);
-                    rs = fmaf(w[n][j], inv_v[n][j], rs);
-                }
-            l[h] = l[h] * corr[h] + rs;                       // (this lane's keys; the lanes of a row are added at the end)
-            m[h] = mn;
-            pf[h] = dq_pack_half(w[0][0], w[0][1]);
-            pf[2 + h] = dq_pack_half(w[1][0], w[1][1]);
-        }
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-            for (int t = 0; t < DQ_NT; ++t) o[t][0] *= corr[0], o[t][1] *= corr[0], o[t][2] *= corr[1], o[t][3] *= corr[1];
-        }
-        // ---- P.V: this lane's four keys, DQ_VB columns at a time
-#pragma unroll
-        for (int vb = 0; vb < DQ_NVB; ++vb) {
-            uint32_t x[4][DQ_VB / 4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int key = 2 * lq + (k & 1) + 8 * (k >> 1), col = vb * 8 * DQ_VB + lg * DQ_VB;
-                const int piece = (key * (DQ_HD / 16) + col / 16) ^ kvq_turn(DQ_HD, true, key);
-                const unsigned char* at = rec + KVQ_PAGE * DQ_HD + piece * 16 + col % 16;
-                if constexpr (DQ_VB == 16) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at);
-                    x[k][0] = w.x, x[k][1] = w.y, x[k][2] = w.z, x[k][3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(at);
-                    x[k][0] = w.x, x[k][1] = w.y;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < DQ_VB / 4; ++i) {
-                uint32_t a[2][2];                             // [keys 2 lq, + 1 | 8 + 2 lq, + 1][columns 0, 1 | 2, 3]: two keys of a column side by side
+            for (int kg = 0; kg < DQ_KG; ++kg) {
+                uint32_t c[2][4];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    a[n][0] = __byte_perm(x[2 * n][i], x[2 * n + 1][i], 0x5140);
-                    a[n][1] = __byte_perm(x[2 * n][i], x[2 * n + 1][i], 0x7362);
-                    if (edge) a[n][0] &= seen[n], a[n][1] &= seen[n];
-                    a[n][0] = kvq_raw<KIND>(a[n][0]), a[n][1] = kvq_raw<KIND>(a[n][1]);
+                    const int key = 8 * n + lg, piece = (key * (DQ_HD / 16) + 4 * kg + lq) ^ kvq_turn(DQ_HD, false, key);
+                    const uint4 w = *reinterpret_cast<const uint4*>(rec + piece * 16);
+                    c[n][0] = w.x, c[n][1] = w.y, c[n][2] = w.z, c[n][3] = w.w;
                 }
-                const int t = vb * DQ_VB + 4 * i;
-                dq_mma(o[t], pf, kvq_low<KIND>(a[0][0]), kvq_low<KIND>(a[1][0]));
-                dq_mma(o[t + 1], pf, kvq_high<KIND>(a[0][0]), kvq_high<KIND>(a[1][0]));
-                dq_mma(o[t + 2], pf, kvq_low<KIND>(a[0][1]), kvq_low<KIND>(a[1][1]));
-                dq_mma(o[t + 3], pf, kvq_high<KIND>(a[0][1]), kvq_high<KIND>(a[1][1]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a[4];
+                    dq_halves<KIND>(c[0][i], a[0], a[2]);
+                    dq_halves<KIND>(c[1][i], a[1], a[3]);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) dq_mma(i & 1 ? s1[j] : s[j], a, qf[4 * kg + i][j][0], qf[4 * kg + i][j][1]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[j][i] += s1[j][i];
+            // ---- exponents of this lane's two keys, softmax in base 2, two heads an instruction. K's power and V's inverse power are made one unit of 2^-23 too large,
+            // so that the byte of a row that is NaN, 255, gives a NaN and not an infinity.
+            const int page0 = (p0 + warp + it * DQ_WARPS) * KVQ_PAGE;
+            const bool gone = (bad >> (it & 31)) & 1, edge = gone || page0 < lo || page0 + KVQ_PAGE > kvlen;
+            float tv[NT][4], inv_v[2];
+            uint32_t seen[2] = {0u, 0u};          // on a page that is not seen whole: the bytes of V's pairs of keys 2 lq, + 1 and 8 + 2 lq, + 1 that count (e4m3 has codes that are NaN)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const uint32_t ke = rec[2 * KVQ_PAGE * DQ_HD + 8 * n + lg], ve = rec[2 * KVQ_PAGE * DQ_HD + KVQ_PAGE + 8 * n + lg];
+                const float kp = __uint_as_float(ke << 23 | 1u), add = __uint_as_float(0x4b000000u | ve) - 8388735.f;     // (2^23 + byte as a float has the byte in its lowest bits)
+                inv_v[n] = __uint_as_float(0x7f000001u - (ve << 23));
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    il_f2_get(il_f2_fma(il_f2_mul(il_f2_make(s[j][2 * n], s[j][2 * n + 1]), il_f2_dup(kp)), s_scale[j], il_f2_dup(add)), tv[j][2 * n], tv[j][2 * n + 1]);
+            }
+            if (edge) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = page0 + 8 * n + 2 * lq + j;
+                        if (!gone && key >= lo && key < kvlen) seen[n] |= j ? 0xff00ff00u : 0x00ff00ffu;
+                    }
+                    const int key = page0 + 8 * n + lg;
+                    if (gone || key < lo || key >= kvlen) {
+                        inv_v[n] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) tv[j][2 * n] = tv[j][2 * n + 1] = -INFINITY;
+                    }
+                }
+            }
+            bool up = false;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) up |= fmaxf(tv[j][0], tv[j][2]) > m[j][0] + DQ_RAISE || fmaxf(tv[j][1], tv[j][3]) > m[j][1] + DQ_RAISE;
+            if (__any_sync(0xffffffffu, up)) {    // also the first keys of a head (m = -inf)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float corr[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float mx = fmaxf(tv[j][i], tv[j][2 + i]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        const float mn = mx > m[j][i] + DQ_RAISE ? mx : m[j][i];
+                        corr[i] = mn == m[j][i] ? 1.f : dq_ex2(m[j][i] - mn);     // 0 when nothing was summed yet
+                        m[j][i] = mn;
+                    }
+                    l[j] = il_f2_mul(l[j], il_f2_make(corr[0], corr[1]));
+#pragma unroll
+                    for (int t = 0; t < DQ_MT; ++t) o[t][j][0] *= corr[0], o[t][j][1] *= corr[1], o[t][j][2] *= corr[0], o[t][j][3] *= corr[1];
+                }
+            }
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float m0 = m[j][0] == -INFINITY ? 0.f : m[j][0], m1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float w0 = dq_ex2(tv[j][2 * n] - m0), w1 = dq_ex2(tv[j][2 * n + 1] - m1);
+                    l[j] = il_f2_fma(il_f2_make(w0, w1), il_f2_dup(inv_v[n]), l[j]);          // (this lane's keys; a head's lanes are added at the end)
+                    pf[j][n] = dq_transpose(dq_pack_half(w0, w1));
+                }
+            }
+            // ---- P.V: four keys of this lane's columns, DQ_VB of them at a time
+#pragma unroll
+            for (int vb = 0; vb < DQ_NVB; ++vb) {
+                uint32_t x[4][DQ_VB / 4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = 2 * lq + (k & 1) + 8 * (k >> 1), col = vb * 8 * DQ_VB + lg * DQ_VB;
+                    const int piece = (key * (DQ_HD / 16) + col / 16) ^ kvq_turn(DQ_HD, true, key);
+                    const unsigned char* at = rec + KVQ_PAGE * DQ_HD + piece * 16 + col % 16;
+                    if constexpr (DQ_VB == 16) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at);
+                        x[k][0] = w.x, x[k][1] = w.y, x[k][2] = w.z, x[k][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(at);
+                        x[k][0] = w.x, x[k][1] = w.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < DQ_VB / 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {             // columns 4 i + 2 c, + 1: two keys of a column side by side
+                        uint32_t a[4];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            uint32_t w = __byte_perm(x[2 * n][i], x[2 * n + 1][i], KIND == KVQ_E4M3 ? (c ? 0x7362 : 0x5140) : (c ? 0x7632 : 0x5410));
+                            if (KIND == KVQ_E4M3 && edge) w &= seen[n];
+                            dq_halves<KIND>(w, a[2 * n], a[2 * n + 1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) dq_mma(o[vb * (DQ_VB / 2) + 2 * i + c][j], a, pf[j][0], pf[j][1]);
+                    }
+            }
+            __syncwarp();
+            issue(it + DQ_STAGES);                // refill the place this record came from
+        }
+        done += n_my;
+        if (at >= to) il_pdl_tail();              // (behind the last stretch's products: what follows may become resident)
+        float lsum[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            il_f2_get(l[j], lsum[j][0], lsum[j][1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) lsum[j][i] += __shfl_xor_sync(0xffffffffu, lsum[j][i], x);
+        }
+        __syncthreads();                          // the rings' memory is reused for the merge
+
+        // The four warps' sums, brought to the heads' common maximum, then added in warp order.
+        float* sm_ml = reinterpret_cast<float*>(smem);                     // [warp][row][m, l]
+        float* sm_o = sm_ml + (DQ_WARPS + 1) * ROWS * 2;                   // behind the rows' own m and l: [warp][row][DQ_OS]
+        if (lg == 0) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    sm_ml[(warp * ROWS + 8 * j + 2 * lq + i) * 2] = m[j][i];
+                    sm_ml[(warp * ROWS + 8 * j + 2 * lq + i) * 2 + 1] = lsum[j][i];
+                }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * j + 2 * lq + i;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, sm_ml[(w * ROWS + r) * 2]);
+                const float f = m[j][i] == -INFINITY ? 0.f : dq_ex2(m[j][i] - M);
+                float* row = sm_o + (size_t)(warp * ROWS + r) * DQ_OS;
+#pragma unroll
+                for (int vb = 0; vb < DQ_NVB; ++vb)
+#pragma unroll
+                    for (int t = 0; t < DQ_VB / 2; t += 2) {
+                        const int tt = vb * (DQ_VB / 2) + t;
+                        *reinterpret_cast<float4*>(row + vb * 8 * DQ_VB + lg * DQ_VB + 2 * t) = make_float4(f * o[tt][j][i], f * o[tt][j][2 + i], f * o[tt + 1][j][i], f * o[tt + 1][j][2 + i]);
+                    }
+            }
+        if (threadIdx.x < ROWS) {
+            const int r = threadIdx.x;
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, sm_ml[(w * ROWS + r) * 2]);
+#pragma unroll
+            for (int w = 0; w < DQ_WARPS; ++w) {
+                const float mw = sm_ml[(w * ROWS + r) * 2];
+                L += (mw == -INFINITY ? 0.f : dq_ex2(mw - M)) * sm_ml[(w * ROWS + r) * 2 + 1];
+            }
+            *reinterpret_cast<float2*>(sm_ml + (DQ_WARPS * ROWS + r) * 2) = make_float2(M, L);
+        }
+        __syncthreads();
+        // final where the whole unit lies in this block, else a part
+        const bool final = start >= from && start + n_pages <= to;
+        const size_t place = 2 * blockIdx.x + (start >= from ? 1 : 0);
+        __nv_bfloat16* out_rows = out + ((size_t)e * nh + head0) * DQ_HD;
+#pragma unroll
+        for (int i = 0; i < ROWS * (DQ_HD / 4); i += DQ_WARPS * 32) {
+            const int idx = i + threadIdx.x, r = idx / (DQ_HD / 4), d = (idx - r * (DQ_HD / 4)) * 4;
+            if (r >= rows_valid) break;
+            const float2 ML = *reinterpret_cast<const float2*>(sm_ml + (DQ_WARPS * ROWS + r) * 2);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < DQ_WARPS; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * ROWS + r) * DQ_OS + d);
+                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            }
+            dq_write(acc, ML.x, ML.y, final ? out_rows : nullptr, o_part + place * ROWS * DQ_HD, ml_part + place * (2 * ROWS), r, d);
+        }
+        __syncthreads();                              // the next stretch's copies come where the merge was
+    }
+    if (!waited) il_pdl_wait();
+    // requests without a key: zeros
+    for (int z = blockIdx.x; z < n_decode; z += n_blocks)
+        if (entry_kvlen[z] <= 0)
+            for (int i = threadIdx.x; i < nh * (DQ_HD / 8); i += DQ_WARPS * 32) *reinterpret_cast<uint4*>(out + (size_t)z * nh * DQ_HD + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// The parts of a row (a head of a request) added up, WPR warps a row: warp w takes parts w, w + WPR, ..., DQM_ROUND loads under way at a time, a lane four columns, with a
+// running maximum over its rounds (a maximum over all parts first would be one more trip to memory); the warps' sums are then added in warp order. Lengths are read before the
+// wait: they were there when the kernel in front, which waits before it ends, began.
+constexpr int DQM_ROUND = HEAD_DIM > 128 ? 8 : 16;
+template <int WPR>
+__global__ void __launch_bounds__(WPR > 4 ? WPR * 32 : 128) attn_decode_quant_merge_kernel(const float* o_part, const float* ml_part, const int* __restrict__ entry_kvlen, int n_decode,
+                                                                                          int nh, int G, int rows, int row_tiles, int units, int window, int n_blocks, __nv_bfloat16* out) {
+    constexpr int PER = WPR > 4 ? 1 : 4 / WPR;    // rows of a block
+    constexpr int LPR = DQ_HD / 4 < 32 ? DQ_HD / 4 : 32, PPW = 32 / LPR;      // lanes that a part's row takes; the others take the next part of the warp
+    constexpr int NC = DQ_HD > 128 ? 2 : 1;
+    __shared__ float comb[WPR > 1 ? WPR * DQ_HD : 1];
+    __shared__ float2 sums[WPR > 1 ? WPR : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR, row = blockIdx.x * PER + warp / WPR;
+    const bool there = row < n_decode * nh;
+    const int e = there ? row / nh : 0, h = row - e * nh;
+    const int head = h / G, rt = (h - head * G) / rows, r = h - head * G - rt * rows;
+    const DqDeal d = dq_deal(entry_kvlen, n_decode, window, units, n_blocks, 0, lane);
+    int before = 0, first;
+    for (int i = lane; i < e; i += 32) before += dq_pages(entry_kvlen[i], window, &first);
+    before = __reduce_add_sync(0xffffffffu, before) * units;
+    const int n = there ? dq_pages(entry_kvlen[e], window, &first) : 0, start = before + (head * row_tiles + rt) * n;
+    const int b0 = start / d.share, n_parts = n > 0 ? (start + n - 1) / d.share - b0 + 1 : 0;
+    il_pdl_wait();
+    if (n_parts <= 1) return;                     // final already (all warps of a row alike; with more than one warp a row, the block)
+    float acc[NC][4], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+    const int d0 = lane % LPR * 4;
+    for (int i0 = sub * PPW + lane / LPR; i0 < n_parts; i0 += DQM_ROUND * WPR * PPW) {
+        float4 v[NC][DQM_ROUND];
+        float2 ml[DQM_ROUND];
+#pragma unroll
+        for (int k = 0; k < DQM_ROUND; ++k) {     // (behind the last part: a part that is there, counted with factor 0; loads behind a branch would wait for one another)
+            const int i = i0 + k * WPR * PPW;
+            const size_t at = (size_t)dq_place(b0, i < n_parts ? i : i0) * rows + r;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) v[c][k] = *reinterpret_cast<const float4*>(o_part + at * DQ_HD + 128 * c + d0);
+            ml[k] = *reinterpret_cast<const float2*>(ml_part + at * 2);
+            if (i >= n_parts) ml[k] = make_float2(-INFINITY, 0.f);
+        }
+        float mx = M;
+#pragma unroll
+        for (int k = 0; k < DQM_ROUND; ++k) mx = fmaxf(mx, ml[k].x);
+        const float corr = M == -INFINITY ? 0.f : dq_ex2(M - mx);
+        M = mx, L *= corr;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c][0] *= corr, acc[c][1] *= corr, acc[c][2] *= corr, acc[c][3] *= corr;
+#pragma unroll
+        for (int k = 0; k < DQM_ROUND; ++k) {
+            const float f = ml[k].x == -INFINITY ? 0.f : dq_ex2(ml[k].x - M);
+            L += f * ml[k].y;                     // (a NaN of a part that is there stays one)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[c][0] += f * v[c][k].x, acc[c][1] += f * v[c][k].y, acc[c][2] += f * v[c][k].z, acc[c][3] += f * v[c][k].w;
+        }
+    }
+#pragma unroll
+    for (int x = LPR; x < 32; x <<= 1) {          // lanes that had other parts of the same columns
+        const float Mo = __shfl_xor_sync(0xffffffffu, M, x), mx = fmaxf(M, Mo), f = M == -INFINITY ? 0.f : dq_ex2(M - mx);
+        L *= f, L += __shfl_xor_sync(0xffffffffu, L, x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[0][c] *= f, acc[0][c] += __shfl_xor_sync(0xffffffffu, acc[0][c], x);
+        M = mx;
+    }
+    if constexpr (WPR > 1) {
+        if (lane < LPR)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) *reinterpret_cast<float4*>(comb + sub * DQ_HD + 128 * c + d0) = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
+        if (lane == 0) sums[sub] = make_float2(M, L);
+        __syncthreads();
+        if (sub) return;
+        float f[WPR];
+        M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) M = fmaxf(M, sums[w].x);
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) f[w] = sums[w].x == -INFINITY ? 0.f : dq_ex2(sums[w].x - M), L += f[w] * sums[w].y;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(comb + w * DQ_HD + 128 * c + d0);
+                acc[c][0] += f[w] * v.x, acc[c][1] += f[w] * v.y, acc[c][2] += f[w] * v.z, acc[c][3] += f[w] * v.w;
             }
         }
-        __syncwarp();
-        issue(it + DQ_STAGES);                    // refill the stage this record came from
     }
+    if (lane >= LPR) return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    }
-    __syncthreads();                              // the pipeline memory is reused for the merge
-
-    // The four warps' sums, brought to the rows' common maximum, then added in warp order.
-    float* sm_ml = reinterpret_cast<float*>(smem);                     // [warp][16 rows][m, l]
-    float* sm_o = sm_ml + DQ_WARPS * 16 * 2;                           // [warp][16 rows][DQ_OS]
-    if (lq == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            sm_ml[(warp * 16 + lg + 8 * h) * 2] = m[h];
-            sm_ml[(warp * 16 + lg + 8 * h) * 2 + 1] = l[h];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = lg + 8 * h;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
-        const float f = m[h] == -INFINITY ? 0.f : dq_ex2(m[h] - M);
-        float* row = sm_o + (size_t)(warp * 16 + r) * DQ_OS;
-#pragma unroll
-        for (int vb = 0; vb < DQ_NVB; ++vb)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)           // tile columns 2 lq + j: columns DQ_VB (2 lq + j) .. of this block of columns
-#pragma unroll
-                for (int t = 0; t < DQ_VB; t += 4)
-                    *reinterpret_cast<float4*>(row + vb * 8 * DQ_VB + (2 * lq + j) * DQ_VB + t) =
-                        make_float4(f * o[vb * DQ_VB + t][2 * h + j], f * o[vb * DQ_VB + t + 1][2 * h + j], f * o[vb * DQ_VB + t + 2][2 * h + j],
-                                    f * o[vb * DQ_VB + t + 3][2 * h + j]);
-    }
-    il_pdl_tail();
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < rows_valid * (DQ_HD / 4); idx += DQ_WARPS * 32) {
-        const int r = idx / (DQ_HD / 4), d = (idx - r * (DQ_HD / 4)) * 4;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < DQ_WARPS; ++w) M = fmaxf(M, sm_ml[(w * 16 + r) * 2]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < DQ_WARPS; ++w) {
-            const float mw = sm_ml[(w * 16 + r) * 2];
-            L += (mw == -INFINITY ? 0.f : dq_ex2(mw - M)) * sm_ml[(w * 16 + r) * 2 + 1];
-            const float4 v = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * 16 + r) * DQ_OS + d);
-            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-        }
-        const size_t row = (size_t)e * nh + head0 + r;
-        if (out_direct) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;       // (no key seen: zeros)
-            *reinterpret_cast<uint2*>(out_direct + row * DQ_HD + d) = make_uint2(dq_pack_bf16(acc.x * inv, acc.y * inv), dq_pack_bf16(acc.z * inv, acc.w * inv));
-        } else {
-            *reinterpret_cast<float4*>(o_part + (row * n_splits + split) * DQ_HD + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(ml_part + (row * n_splits + split) * 2) = make_float2(M, L);
-        }
-    }
+    for (int c = 0; c < NC; ++c) dq_write(make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]), M, L, out + (size_t)row * DQ_HD, nullptr, nullptr, 0, 128 * c + d0);
 }
 
-// The merge: a warp a (token, head) row, a lane four columns at a time; the splits are added in order.
-__global__ void __launch_bounds__(128) attn_decode_quant_merge_kernel(const float* o_part, const float* ml_part, const int* __restrict__ entry_kvlen, int nh,
-                                                                      int n_rows, int window, int n_splits, __nv_bfloat16* out) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int kvlen = row < n_rows ? entry_kvlen[row / nh] : 0;
-    il_pdl_wait();
-    if (row >= n_rows) return;
-    int n_valid = 0;                              // splits that have keys
-    if (kvlen > 0) {
-        const int n_pages = (kvlen - 1) / KVQ_PAGE - il_mask_lo(kvlen - 1, window) / KVQ_PAGE + 1, per_split = (n_pages + n_splits - 1) / n_splits;
-        n_valid = (n_pages + per_split - 1) / per_split;
-    }
-    const float* ml = ml_part + (size_t)row * n_splits * 2;
-    float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < n_valid; s += 32) M = fmaxf(M, ml[2 * s]);
-    M = il_warp_max(M);
-    for (int s = lane; s < n_valid; s += 32) L += (ml[2 * s] == -INFINITY ? 0.f : dq_ex2(ml[2 * s] - M)) * ml[2 * s + 1];
-    L = il_warp_sum(L);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    for (int d = lane * 4; d < DQ_HD; d += 128) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < n_valid; ++s) {
-            const float f = ml[2 * s] == -INFINITY ? 0.f : dq_ex2(ml[2 * s] - M);
-            const float4 v = *reinterpret_cast<const float4*>(o_part + ((size_t)row * n_splits + s) * DQ_HD + d);
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-        }
-        *reinterpret_cast<uint2*>(out + (size_t)row * DQ_HD + d) = make_uint2(dq_pack_bf16(acc.x * inv, acc.y * inv), dq_pack_bf16(acc.z * inv, acc.w * inv));
-    }
+// Calls go(kernel, shared memory) for the kernel of these.
+template <typename Go>
+static auto dq_pick(int kind, int group, Go go) {
+    if (group <= 8) return kind == KVQ_E4M3 ? go(attn_decode_quant_kernel<KVQ_E4M3, 1>, dq_smem(8)) : go(attn_decode_quant_kernel<KVQ_INT8, 1>, dq_smem(8));
+    return kind == KVQ_E4M3 ? go(attn_decode_quant_kernel<KVQ_E4M3, 2>, dq_smem(16)) : go(attn_decode_quant_kernel<KVQ_INT8, 2>, dq_smem(16));
 }
-
 static int dq_prepare(int dev) {
     static bool done[64];
     if (dev < 0 || dev >= 64 || done[dev]) return IL_OK;
-    cudaError_t e = cudaFuncSetAttribute(attn_decode_quant_kernel<KVQ_E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_decode_quant_kernel<KVQ_INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM);
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+        e = dq_pick(i & 1, i & 2 ? 16 : 1, [](auto kernel, int smem) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (e != cudaSuccess) return 1000 + (int)e;
     done[dev] = true;
     return IL_OK;
 }
 
-// Blocks that this device runs at once; 0 if the query fails. The caller sizes the number of splits by it.
-IL_EXPORT int il_attn_decode_quant_resident_blocks() {
-    int dev = 0, per_sm = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dq_prepare(dev) != IL_OK ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attn_decode_quant_kernel<KVQ_E4M3>, DQ_WARPS * 32, DQ_SMEM) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
+// Blocks that this device runs at once, of either kind of cache, with `group` query heads a kv head; 0 if the query fails.
+IL_EXPORT int il_attn_decode_quant_resident_blocks(int group) {
+    int dev = 0, sms = 0, least = 1 << 20;
+    if (cudaGetDevice(&dev) != cudaSuccess || dq_prepare(dev) != IL_OK || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) least = 0;
+    for (int kind = 0; kind < 2 && least; ++kind) {
+        int n = 0;
+        if (dq_pick(kind, group, [&](auto kernel, int smem) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, DQ_WARPS * 32, smem); }) != cudaSuccess) n = 0;
+        least = n < least ? n : least;
     }
-    return per_sm * sms;
+    if (!least) cudaGetLastError();
+    return least * sms;
 }
 
-// Scratch for more than one split: o_part float32 [n_decode * nh * n_splits * head_dim], ml_part [n_decode * nh * n_splits * 2].
+// n_blocks: blocks that the pages are dealt out to, or 0: a block a unit. Scratch for n_blocks > 0: o_part float32 [2 * n_blocks * 16 * head_dim], ml_part [2 * n_blocks * 32].
 IL_EXPORT int il_attn_decode_quant(const void* q, long long q_stride, void* out, const void* cache, int kind, const int* block_table, int bt_stride,
-                                   const int* entry_kvlen, int n_decode, int nh, int nkv, int hd, float scale, int window, int n_splits, float* o_part,
+                                   const int* entry_kvlen, int n_decode, int nh, int nkv, int hd, float scale, int window, int n_blocks, float* o_part,
                                    float* ml_part, int* status, int early, cudaStream_t stream) {
     if (n_decode <= 0) return IL_OK;
-    if (hd != HEAD_DIM || n_splits > DQ_MAX_SPLITS || n_decode > 65535) return IL_UNSUPPORTED;
-    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_splits <= 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !status) return IL_BAD_ARG;
+    if (hd != HEAD_DIM) return IL_UNSUPPORTED;
+    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !status) return IL_BAD_ARG;
+    const int group = nh / nkv, rows = group <= 8 ? 8 : 16, row_tiles = (group + rows - 1) / rows, units = nkv * row_tiles;
+    if ((long long)n_decode * units * bt_stride > 0x7fffffffLL || n_blocks > 0x3fffffff) return IL_UNSUPPORTED;   // (pages of all units are counted in 32 bits)
+    if (n_blocks > 0 && (!o_part || !ml_part)) return IL_BAD_ARG;
     if ((((uintptr_t)cache | (uintptr_t)q | (uintptr_t)out) & 15) || (q_stride & 7) || q_stride < (long long)nh * hd) return IL_BAD_ARG;
-    const int row_tiles = (nh / nkv + 15) / 16;
-    if ((long long)nkv * row_tiles > 65535) return IL_UNSUPPORTED;
     int dev = 0;
     cudaGetDevice(&dev);
     const int rc = dq_prepare(dev);
     if (rc != IL_OK) return rc;
-    const dim3 grid(n_splits, nkv * row_tiles, n_decode);
-    __nv_bfloat16* direct = n_splits == 1 ? (__nv_bfloat16*)out : nullptr;
-#define DQ_GO(KIND)                                                                                                                               \
-    IL_LAUNCH((attn_decode_quant_kernel<KIND>), grid, DQ_WARPS * 32, DQ_SMEM, stream, (const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache, \
-              block_table, bt_stride, entry_kvlen, nh, nkv, scale * 1.4426950408889634f, window, n_splits, o_part, ml_part, direct, status, early)
-    if (kind == KVQ_E4M3) DQ_GO(KVQ_E4M3);
-    else DQ_GO(KVQ_INT8);
-#undef DQ_GO
-    if (n_splits > 1) {
-        const int n_rows = n_decode * nh;
-        IL_LAUNCH(attn_decode_quant_merge_kernel, (n_rows + 3) / 4, 128, 0, stream, (const float*)o_part, (const float*)ml_part, entry_kvlen, nh, n_rows,
-                  window, n_splits, (__nv_bfloat16*)out);
+    const int whole = n_blocks == 0;
+    cudaError_t e = dq_pick(kind, group, [&](auto kernel, int smem) {
+        return il_launch(kernel, dim3(whole ? n_decode * units : n_blocks), dim3(DQ_WARPS * 32), (size_t)smem, stream, (const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache, block_table, bt_stride,
+                         entry_kvlen, n_decode, nh, nkv, group, row_tiles, scale * 1.4426950408889634f, window, whole, o_part, ml_part, (__nv_bfloat16*)out, status, early);
+    });
+    if (e == cudaSuccess && !whole) {
+        // warps a row by the parts that a unit has if the requests are alike
+        const int parts = n_blocks / (n_decode * units), n_rows = n_decode * nh;
+        const auto merge = [&](auto kernel, int blocks, int threads) {
+            return il_launch(kernel, dim3(blocks), dim3(threads), (size_t)0, stream, (const float*)o_part, (const float*)ml_part, entry_kvlen, n_decode, nh, group, rows, row_tiles, units, window, n_blocks,
+                             (__nv_bfloat16*)out);
+        };
+        e = parts > 64 ? merge(attn_decode_quant_merge_kernel<16>, n_rows, 512) : parts > 8 ? merge(attn_decode_quant_merge_kernel<4>, n_rows, 128)
+                                                                                : merge(attn_decode_quant_merge_kernel<1>, (n_rows + 3) / 4, 128);
     }
+    if (e != cudaSuccess) return 1000 + (int)e;
     IL_LAUNCH_CHECK();
     return IL_OK;
 }

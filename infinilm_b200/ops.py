@@ -1919,19 +1919,27 @@ def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_k
 
 
 _resident_quant = {}
+# A block a unit, with every sum final, where dealing the pages out would take less than so many of them off the longest block: the second kernel then costs more than it
+# saves. Dealt out / whole, us: 64 requests of 256 tokens (16 pages), 32 heads on 8 of 128, 15.8 / 9.4; of 512 19.9 / 13.9; one request of 256, 32 heads on 2, 7.5 / 7.5, of 512
+# (24 pages less) 8.6 / 10.4.
+QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES = 8, 12
 
 
-def _quant_splits(head_dim: int, base: int, pages: int) -> int:
-    """Splits of the keys for `base` blocks a split: as many as fill two thirds of what the device runs at once, at least four pages a split."""
-    key = (_cur_device(), head_dim)
-    n = _resident_quant.get(key)
-    if n is None:
+def _quant_blocks(head_dim: int, group: int, units: int, pages: int) -> int:
+    """Blocks that the pages of `units` units (a kv head of a request with up to 8 or 16 of its `group` query heads) of at most `pages` pages are dealt out to: one wave of
+    them, eight pages each at least; 0: a block a unit."""
+    key = (_cur_device(), head_dim, group > 8)
+    most = _resident_quant.get(key)
+    if most is None:
         fn = build.load("attn_decode_quant", {"HEAD_DIM": head_dim}).il_attn_decode_quant_resident_blocks
-        fn.argtypes, fn.restype = [], _c_int
-        n = _resident_quant[key] = int(fn())
-        if n <= 0:
+        fn.argtypes, fn.restype = [_c_int], _c_int
+        most = _resident_quant[key] = int(fn(group))
+        if most <= 0:
             raise KernelError("attention_decode_quant: the occupancy query failed")
-    return max(1, min(n * 2 // 3 // base, (pages + 3) // 4, 128))
+    least = QUANT_LEAST_PAGES
+    if pages <= QUANT_WHOLE_PAGES + max(least, units * pages // most):
+        return 0
+    return min(most, units * ((pages + least - 1) // least))
 
 
 def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_kvlen: torch.Tensor,
@@ -1940,8 +1948,8 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     """Attention of one new token a request over an 8-bit cache: row i of `q` (bfloat16 [rows, >= heads * head_dim], the queries in its first columns) is entry i's
     token at position entry_kvlen[i] - 1 and sees the keys up to itself, of the last `window` positions if given (negative: of its run of -window positions).
     `out` bfloat16 [rows, heads * head_dim]; head_dim 64, 128 or 256. A row that sees no key gets zeros; a block-table entry below 0 is never followed, its keys count as masked.
-    max_kvlen: no entry is longer (what the split over the keys is planned for; a larger bound costs time, not results' correctness).
-    ws: a `Workspace` for the splits' partial sums. cached_before: the caller vouches that lengths, block tables and all pages but the newest token's were written before
+    max_kvlen: no entry is longer (what the number of blocks is planned for; any bound gives right results).
+    ws: a `Workspace` for the parts of sums that several blocks make. cached_before: the caller vouches that lengths, block tables and all pages but the newest token's were written before
     the kernel in front of this call began; they are then read while that kernel still runs."""
     what = "attention_decode_quant"
     if n_decode <= 0:
@@ -1958,19 +1966,19 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries]")
     _on_one_device(what, q, out, cache, block_table, entry_kvlen)
     w = int(window or 0)
-    seen = max(1, int(max_kvlen)) if not w else max(1, min(int(max_kvlen), abs(w) + KV_QUANT_PAGE))
-    n_splits = _quant_splits(head_dim, n_decode * n_kv_heads * ((n_heads // n_kv_heads + 15) // 16), (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE)
+    seen = max(1, int(max_kvlen)) if not w else max(1, min(int(max_kvlen), abs(w) + KV_QUANT_PAGE))       # (a window may begin inside a page)
+    group = n_heads // n_kv_heads
+    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE)
     o_part = ml_part = None
-    if n_splits > 1:
-        rows = n_decode * n_heads * n_splits
-        o_part, ml_part = ws.flat("quant_o_part", rows * head_dim, torch.float32), ws.flat("quant_ml_part", rows * 2, torch.float32)
+    if n_blocks > 0:
+        o_part, ml_part = ws.flat("quant_o_part", n_blocks * 32 * head_dim, torch.float32), ws.flat("quant_ml_part", n_blocks * 64, torch.float32)
     f = _fn("attn_decode_quant", "il_attn_decode_quant", [_c_void_p, _c_ll, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
                                                           _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p],
             defines={"HEAD_DIM": head_dim})
     _check(f(_ptr(q), q.stride(0), _ptr(out), _ptr(cache), k, _ptr(block_table), block_table.shape[1], _ptr(entry_kvlen), n_decode, n_heads, n_kv_heads, head_dim,
-             scale, w, n_splits, _ptr(o_part), _ptr(ml_part), _ptr(stream_status(q.device)), int(cached_before), _stream()), what)
-    if n_splits > 1:
-        count_launches(1)                         # the merge kernel
+             scale, w, n_blocks, _ptr(o_part), _ptr(ml_part), _ptr(stream_status(q.device)), int(cached_before), _stream()), what)
+    if n_blocks > 0:
+        count_launches(1)                         # the second kernel
 
 
 def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:

@@ -239,9 +239,9 @@ def _decode_check(out, q, val, rows, kvlens, nh, hd, scale, window):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 64), (4, 4, 64), (32, 2, 128), (6, 2, 128), (20, 1, 128), (8, 2, 256), (40, 1, 64)])
-@pytest.mark.parametrize("splits", [1, 2, 7, 128])
+@pytest.mark.parametrize("blocks", [0, 1, 2, 7, 300])
 @pytest.mark.parametrize("window", [None, 20, -24])
-def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, splits, window):
+def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, window):
     ops, dev = _ops(), cuda_device
     kvlens = [300, 1, 0, 16, 17, 129, 15, 47]
     rows, n_pages = _tables(kvlens, 3, 6)
@@ -255,7 +255,7 @@ def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, splits, 
     q = (2 * torch.randn((len(kvlens), nh * hd), generator=g)).to(torch.bfloat16)
     q[:, :hd] *= 2.0 ** 20                        # a head far outside what a half holds
     q[:, hd:2 * hd] *= 2.0 ** -30
-    monkeypatch.setattr(ops, "_quant_splits", lambda *a: splits)
+    monkeypatch.setattr(ops, "_quant_blocks", lambda *a: blocks)
     out = torch.full((len(kvlens), nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
     scale = 0.7 / math.sqrt(hd)
     for early in (False, True):
@@ -267,8 +267,8 @@ def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, splits, 
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128, 256])
-@pytest.mark.parametrize("splits", [1, 5])
-def test_decode_pages_that_are_not_there_and_rows_that_are_not_finite(cuda_device, monkeypatch, kind, hd, splits):
+@pytest.mark.parametrize("blocks", [0, 5, 23])
+def test_decode_pages_that_are_not_there_and_rows_that_are_not_finite(cuda_device, monkeypatch, kind, hd, blocks):
     """A missing page's keys are masked, a request without any page gets zeros; a NaN row reaches the heads and requests that see it, no others; exponents far apart."""
     ops, dev = _ops(), cuda_device
     nh, nkv, kvlens = 4, 2, [70, 40, 33, 64, 90]
@@ -286,7 +286,7 @@ def test_decode_pages_that_are_not_there_and_rows_that_are_not_finite(cuda_devic
     rec[rows[2][0], 1, 32 * hd + 16 + 3] = 255    # V of kv head 1, key 3 of request 2: NaN
     rec[rows[3][1], 0, 32 * hd + 7] = 255         # K of kv head 0, key 23 of request 3: NaN
     q = torch.randn((5, nh * hd), generator=g).to(torch.bfloat16)
-    monkeypatch.setattr(ops, "_quant_splits", lambda *a: splits)
+    monkeypatch.setattr(ops, "_quant_blocks", lambda *a: blocks)
     out = torch.full((5, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
 
     def go(window):
@@ -318,6 +318,26 @@ def test_decode_takes_rows_with_a_stride_and_is_repeatable(cuda_device):
         outs.append(out)
     assert all(torch.equal(o, outs[0]) for o in outs[1:])
     ops.check_status(dev)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("blocks", [16, 17, 100, 600])
+def test_decode_of_long_contexts_in_many_parts(cuda_device, monkeypatch, kind, hd, blocks):
+    """Parts by the hundred of one unit, beside requests of a page; the same bits twice."""
+    ops, dev = _ops(), cuda_device
+    nh, nkv, kvlens = 2, 1, [3, 5000, 16, 2001]
+    rows, n_pages = _tables(kvlens, 2, 18)
+    rec, val = _cache(n_pages, nkv, hd, kind, 19)
+    q = torch.randn((4, nh * hd), generator=torch.Generator().manual_seed(20)).to(torch.bfloat16)
+    monkeypatch.setattr(ops, "_quant_blocks", lambda *a: blocks)
+    ws, outs = _ws(dev), []
+    for _ in range(2):
+        out = torch.full((4, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
+        ops.attention_decode_quant(q.to(dev), out, rec.to(dev), kind, _i32(rows, dev), _i32(kvlens, dev), 4, nh, nkv, hd, 0.1, None, 5000, ws)
+        outs.append(out.cpu())
+    assert torch.equal(outs[0], outs[1])
+    _decode_check(outs[0], q, val, rows, kvlens, nh, hd, 0.1, 0)
 
 
 def test_offsets_past_32_bits(cuda_device):
