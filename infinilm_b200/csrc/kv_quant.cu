@@ -6,6 +6,8 @@
 // may be the same place.
 // il_kv_unpack: pages of requests as pages of bfloat16 or float32 values in the layout of the plain cache, [page][K, V][kv head][16][head_dim].
 // Both are bound by memory: what they read and write is named at each kernel.
+#include <algorithm>
+
 #include "kv_quant.cuh"
 
 // Angle of one pair: cos and sin, times mscale. The product is exact in 64 bits (24 bits by 31), the reduction by whole turns leaves an error near 1e-16 times the turns.
@@ -20,6 +22,133 @@ __device__ __forceinline__ void kvq_angle(int pos, float freq, float mscale, flo
 // The products are rounded one by one, so that the code does not depend on how the compiler joins them.
 __device__ __forceinline__ float kvq_lo(float x1, float x2, float c, float s) { return __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)); }
 __device__ __forceinline__ float kvq_hi(float x1, float x2, float c, float s) { return __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)); }
+
+template <typename TA> struct KvqEight { uint4 w[sizeof(TA) / 2]; };           // eight elements: one 16-byte load, or two
+template <typename TA>
+__device__ __forceinline__ KvqEight<TA> kvq_load8(const TA* p) {
+    KvqEight<TA> v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(TA) / 2; ++i) v.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return v;
+}
+template <typename TA>
+__device__ __forceinline__ void kvq_store8(TA* p, const float (&x)[8]) {
+    KvqEight<TA> v;
+    TA* e = reinterpret_cast<TA*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = il_from_f<TA>(x[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(TA) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v.w[i];
+}
+template <int KIND>
+__device__ __forceinline__ uint2 kvq_codes8(const float (&x)[8], float f) {
+    return make_uint2(kvq_codes4<KIND>(x[0] * f, x[1] * f, x[2] * f, x[3] * f), kvq_codes4<KIND>(x[4] * f, x[5] * f, x[6] * f, x[7] * f));
+}
+
+// Where the rotated pairs come in whole runs of eight: a lane takes 16 columns of a head, eight and the eight they turn with (or 16 neighbours of v and of what is
+// not turned), PER lanes (a power of two) a head, which agree on the head's exponent by shuffles, 32 / PER heads of one token a warp at a time. A lane's columns are the same in every
+// head, so its eight angles are made once; the lanes of a warp that need the same ones make them together. One pass, each element read once and written once; bound by
+// memory, so what matters is loads under way: the next round's while one is worked on, no barrier, registers for four blocks an SM (more rounds ahead with fewer blocks: 65 to 78 us for
+// what takes 61). `wpt`: warps a token, many where the tokens are few. 9,420 tokens, 32 heads on 8 of
+// 128, bfloat16, us: 230 with a column a lane at a time, 103 with a block a token and its angles in shared memory, 43 so.
+constexpr int KVS_AHEAD = 1, KVS_WARPS = 148 * 16;
+template <typename TA, int KIND, int PER>
+__global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* __restrict__ tok_pos,
+                                                               const int* __restrict__ tok_entry, const int* __restrict__ block_table, int bt_stride,
+                                                               unsigned char* cache, int T, int nh, int nkv, int hd, int rot, const float* __restrict__ inv_freq, float mscale,
+                                                               int wpt) {
+    constexpr int HEADS = 32 / PER, OWN = 8 / HEADS > 0 ? 8 / HEADS : 1;      // heads of a round, angles that a lane makes
+    il_pdl_begin();
+    const int lane = threadIdx.x & 31, j = lane % PER, g = lane / PER;
+    const int gw = blockIdx.x * 8 + (threadIdx.x >> 5), t = gw / wpt, part = gw - t * wpt;
+    if (t >= T) return;
+    const int half = rot >> 1, pairs = rot >> 4, lanes = hd >> 4, rows = cache ? nh + 2 * nkv : nh, pos = tok_pos[t];
+    const TA* row0 = qkv + t * row_stride;
+    TA* to0 = q_out + t * q_stride;
+    unsigned char* page = nullptr;                // kv head 0's record; null: not stored
+    if (cache) {
+        const int id = block_table[(size_t)tok_entry[t] * bt_stride + pos / KVQ_PAGE];
+        if (id >= 0) page = cache + (size_t)id * nkv * kvq_record(hd);            // the host reserves every page a step touches; never write elsewhere
+    }
+    const int key = pos % KVQ_PAGE;
+    KvqEight<TA> va[KVS_AHEAD], vb[KVS_AHEAD];
+    const auto place = [&](int r, int& a, int& b) {           // columns a .. a + 7 and b .. b + 7
+        const bool turns = r < nh + nkv && j < pairs;
+        a = turns ? j * 8 : j * 16, b = turns ? a + half : a + 8;
+        return turns;
+    };
+    const auto load = [&](int first) {
+#pragma unroll
+        for (int u = 0; u < KVS_AHEAD; ++u) {
+            const int r = first + u * wpt * HEADS + g;
+            int a, b;
+            place(r, a, b);
+            if (r < rows && j < lanes) va[u] = kvq_load8(row0 + (size_t)r * hd + a), vb[u] = kvq_load8(row0 + (size_t)r * hd + b);
+        }
+    };
+    load(part * HEADS);                           // on their way while the angles are made
+    float c[8], s[8];
+    if (rot) {
+        float co[OWN], so[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const int at = j * 8 + (g * OWN + i) % 8;
+            co[i] = so[i] = 0.f;
+            if (j < pairs) kvq_angle(pos, inv_freq[at], mscale, &co[i], &so[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = __shfl_sync(0xffffffffu, co[i % OWN], i / OWN * PER + j), s[i] = __shfl_sync(0xffffffffu, so[i % OWN], i / OWN * PER + j);
+    }
+    for (int first = part * HEADS; first < rows; first += KVS_AHEAD * wpt * HEADS) {
+        KvqEight<TA> wa[KVS_AHEAD], wb[KVS_AHEAD];
+#pragma unroll
+        for (int u = 0; u < KVS_AHEAD; ++u) wa[u] = va[u], wb[u] = vb[u];
+        load(first + KVS_AHEAD * wpt * HEADS);
+#pragma unroll
+        for (int u = 0; u < KVS_AHEAD; ++u) {
+            const int r0 = first + u * wpt * HEADS, r = r0 + g;
+            if (r0 >= rows) break;
+            const bool mine = r < rows && j < lanes;
+            int a, b;
+            const bool turns = place(r, a, b);
+            float x[8], y[8];
+            const TA *pa = reinterpret_cast<const TA*>(&wa[u]), *pb = reinterpret_cast<const TA*>(&wb[u]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = il_to_f(pa[i]), y[i] = il_to_f(pb[i]);
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x1 = x[i], x2 = y[i];
+                    x[i] = kvq_lo(x1, x2, c[i], s[i]), y[i] = kvq_hi(x1, x2, c[i], s[i]);
+                }
+            }
+            if (mine && r < nh) {
+                TA* to = to0 + (size_t)r * hd;
+                kvq_store8(to + a, x), kvq_store8(to + b, y);
+            }
+            if (r0 + HEADS <= nh || !page) continue;          // (the warp's heads are all queries)
+            uint32_t most = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, max(__float_as_uint(x[i]) & 0x7fffffffu, __float_as_uint(y[i]) & 0x7fffffffu));
+            if (!mine) most = 0u;
+#pragma unroll
+            for (int o = 1; o < PER; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (!mine || r < nh) continue;
+            const int v = r >= nh + nkv, head = r - nh - v * nkv, e = kvq_exponent<KIND>(most), turn = kvq_turn(hd, v, key), l0 = key * lanes;
+            unsigned char *rec = page + (size_t)head * kvq_record(hd), *plane = rec + v * KVQ_PAGE * hd;
+            const float f = kvq_inverse(e);
+            uint2 ca = make_uint2(0u, 0u), cb = ca;
+            if (e != KVQ_NAN) ca = kvq_codes8<KIND>(x, f), cb = kvq_codes8<KIND>(y, f);
+            if (!turns) {                         // 16 neighbours: one piece
+                *reinterpret_cast<uint4*>(plane + (((l0 + a / 16) ^ turn) << 4)) = make_uint4(ca.x, ca.y, cb.x, cb.y);
+            } else {
+                *reinterpret_cast<uint2*>(plane + (((l0 + a / 16) ^ turn) << 4) + (a & 8)) = ca;
+                *reinterpret_cast<uint2*>(plane + (((l0 + b / 16) ^ turn) << 4) + (b & 8)) = cb;
+            }
+            if (j == 0) rec[2 * KVQ_PAGE * hd + v * KVQ_PAGE + key] = (unsigned char)e;
+        }
+    }
+}
 
 // A warp a row (a head of q, k or v of one token), a lane the columns lane, lane + 32, ...: any even rot, any alignment.
 template <typename TA, int KIND>
@@ -79,6 +208,36 @@ IL_EXPORT int il_rope_store_quant(const void* qkv, int act_kind, long long row_s
     if (nh <= 0 || nkv <= 0 || hd <= 0 || hd % 16 || rot < 0 || rot > hd || (rot & 1) || (rot && !inv_freq)) return IL_BAD_ARG;
     if (row_stride < (long long)(nh + 2 * nkv) * hd || q_stride < (long long)nh * hd || ((uintptr_t)cache & 15)) return IL_BAD_ARG;
     if ((kind != KVQ_E4M3 && kind != KVQ_INT8) || (act_kind != IL_F32 && act_kind != IL_BF16)) return IL_BAD_ARG;
+    const int sz = act_kind == IL_F32 ? 4 : 2;
+    if (rot % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out) & 15) && (row_stride * sz) % 16 == 0 && (q_stride * sz) % 16 == 0) {
+        const int per = hd <= 16 ? 1 : hd <= 32 ? 2 : hd <= 64 ? 4 : hd <= 128 ? 8 : 16, rows = cache ? nh + 2 * nkv : nh;
+        // a warp a round of heads where the tokens are few, as few warps a token as fill the device twice where they are many
+        const int rounds = (rows * per + 31) / 32, wpt = (long long)T * rounds <= KVS_WARPS ? rounds : (int)std::min<long long>(std::max<long long>(KVS_WARPS / T, 1), rounds);
+        const long long warps = (long long)T * wpt;
+        if (warps > 0x7fffffffLL * 8 - 8) return IL_UNSUPPORTED;
+#define KVS_GO(TA, KIND, PER)                                                                                                                                   \
+    IL_LAUNCH((rope_store_quant_kernel<TA, KIND, PER>), (unsigned)((warps + 7) / 8), 256, 0, stream, (const TA*)qkv, row_stride, (TA*)q_out, q_stride, tok_pos, \
+              tok_entry, block_table, bt_stride, (unsigned char*)cache, T, nh, nkv, hd, rot, inv_freq, mscale, wpt)
+#define KVS_PER(TA, KIND)                                \
+    do {                                                 \
+        if (per == 1) KVS_GO(TA, KIND, 1);               \
+        else if (per == 2) KVS_GO(TA, KIND, 2);          \
+        else if (per == 4) KVS_GO(TA, KIND, 4);          \
+        else if (per == 8) KVS_GO(TA, KIND, 8);          \
+        else KVS_GO(TA, KIND, 16);                       \
+    } while (0)
+        if (act_kind == IL_F32) {
+            if (kind == KVQ_E4M3) KVS_PER(float, KVQ_E4M3);
+            else KVS_PER(float, KVQ_INT8);
+        } else {
+            if (kind == KVQ_E4M3) KVS_PER(__nv_bfloat16, KVQ_E4M3);
+            else KVS_PER(__nv_bfloat16, KVQ_INT8);
+        }
+#undef KVS_PER
+#undef KVS_GO
+        IL_LAUNCH_CHECK();
+        return IL_OK;
+    }
     const long long items = (long long)T * (cache ? nh + 2 * nkv : nh), blocks = (items + 7) / 8;
     if (blocks > 0x7fffffffLL) return IL_UNSUPPORTED;
 #define KVS_GO(TA, KIND)                                                                                                                                     \
@@ -96,65 +255,83 @@ IL_EXPORT int il_rope_store_quant(const void* qkv, int act_kind, long long row_s
     return IL_OK;
 }
 
-// A block a page of a request. first: the page of the lowest position that the request's portion sees (its first new token's, by the mask); pages in
-// front of it and behind the last are left as they are, slots behind the request's end become zeros. A thread makes 16 bytes of output at a time.
-template <typename TO, int KIND>
+// A block a page of a request. Pages in front of the one that holds the lowest position the request's portion sees (its first new token's, by the mask) and behind the last
+// are left as they are, slots behind the request's end become zeros. A thread makes 16 bytes of output at a time, KVU_AHEAD of them at once: bound by memory, what matters is loads under
+// way. HD 0: any head size. 16 requests of up to 8,192 tokens, 8 kv heads of 128, e4m3 to bfloat16, us: one at a time 85.4,
+// two 80.2, four 79.9.
+constexpr int KVU_AHEAD = 4;
+template <typename TO, int KIND, int HD>
 __global__ void __launch_bounds__(256) kv_unpack_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
-                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd, TO* pages, int* table, int poison) {
+                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key) {
     il_pdl_begin();
     constexpr int VEC = 16 / sizeof(TO);
+    const int hd = HD ? HD : hd_arg;
     const int i = blockIdx.y, e = first_entry + i, p = blockIdx.x;
     const size_t to = (size_t)i * gridDim.x + p;
     if (table && threadIdx.x == 0) table[(size_t)e * gridDim.x + p] = (int)to;
     const int kvlen = entry_kvlen[e];
     const int lo = entry_qstart ? il_mask_lo(max(kvlen - (entry_qstart[e + 1] - entry_qstart[e]), 0), window) : 0;
-    if (p < lo / KVQ_PAGE || p * KVQ_PAGE >= kvlen) return;
+    if (p < lo / KVQ_PAGE || p >= (kvlen + KVQ_PAGE - 1) / KVQ_PAGE) return;
     const int page = block_table[(size_t)e * bt_stride + p], rec_bytes = kvq_record(hd), n_keys = page < 0 ? 0 : min(KVQ_PAGE, kvlen - p * KVQ_PAGE);
     const unsigned char* recs = cache + (size_t)max(page, 0) * nkv * rec_bytes;
     TO* out = pages + to * 2 * nkv * KVQ_PAGE * hd;
     const int per = hd / VEC, total = 2 * nkv * KVQ_PAGE * per;
-    for (int u = threadIdx.x; u < total; u += 256) {
-        const int row = u / per, d = (u - row * per) * VEC, key = row % KVQ_PAGE, vh = row / KVQ_PAGE, v = vh >= nkv, head = vh - v * nkv;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (key < n_keys) {
-            const unsigned char* rec = recs + (size_t)head * rec_bytes;
-            const unsigned char* at = rec + v * KVQ_PAGE * hd + (((key * (hd / 16) + d / 16) ^ kvq_turn(hd, v, key)) << 4) + d % 16;
-            const unsigned char* ex = rec + 2 * KVQ_PAGE * hd + key;
-            // for the attention a row of V that is NaN is told by its key (a masked key then leaves no trace: its score is replaced, its value is zero)
-            const bool told = poison && ex[KVQ_PAGE] == KVQ_NAN;
-            const float f = kvq_power(told ? KVQ_NAN : ex[v * KVQ_PAGE]);
-            uint32_t c[VEC / 4];
-            if (VEC == 8) {
-                const uint2 g = *reinterpret_cast<const uint2*>(at);
-                c[0] = g.x, c[VEC / 4 - 1] = g.y;
-            } else {
-                c[0] = *reinterpret_cast<const uint32_t*>(at);
-            }
-            TO* o = reinterpret_cast<TO*>(&w);
+    for (int u0 = threadIdx.x; u0 < total; u0 += 256 * KVU_AHEAD) {
+        uint2 code[KVU_AHEAD];
+        int ke[KVU_AHEAD], ve[KVU_AHEAD];
 #pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) {
-                const uint32_t raw = kvq_raw<KIND>(c[k]), h0 = kvq_low<KIND>(raw), h1 = kvq_high<KIND>(raw);
-                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), bb = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                o[4 * k] = il_from_f<TO>(a.x * f), o[4 * k + 1] = il_from_f<TO>(a.y * f);
-                o[4 * k + 2] = il_from_f<TO>(bb.x * f), o[4 * k + 3] = il_from_f<TO>(bb.y * f);
+        for (int k = 0; k < KVU_AHEAD; ++k) {
+            const int u = u0 + 256 * k, row = u / per, d = (u - row * per) * VEC, key = row % KVQ_PAGE, vh = row / KVQ_PAGE, v = vh >= nkv, head = vh - v * nkv;
+            if (u < total && key < n_keys) {
+                const unsigned char* rec = recs + (size_t)head * rec_bytes;
+                const unsigned char* at = rec + v * KVQ_PAGE * hd + (((key * (hd / 16) + d / 16) ^ kvq_turn(hd, v, key)) << 4) + d % 16;
+                if (VEC == 8) code[k] = *reinterpret_cast<const uint2*>(at);
+                else code[k].x = *reinterpret_cast<const uint32_t*>(at);
+                ke[k] = rec[2 * KVQ_PAGE * hd + key], ve[k] = rec[2 * KVQ_PAGE * hd + KVQ_PAGE + key];
             }
-            if (told && v) w = make_uint4(0u, 0u, 0u, 0u);
         }
-        *reinterpret_cast<uint4*>(out + (size_t)row * hd + d) = w;
+#pragma unroll
+        for (int k = 0; k < KVU_AHEAD; ++k) {
+            const int u = u0 + 256 * k, row = u / per, d = (u - row * per) * VEC, key = row % KVQ_PAGE, v = row / KVQ_PAGE >= nkv;
+            if (u >= total) break;
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (key < n_keys) {
+                // for the attention a row of V that is NaN is told by its key (a masked key then leaves no trace: its score is replaced, its value is zero)
+                const bool told = told_by_key && ve[k] == KVQ_NAN;
+                const float f = kvq_power(told ? KVQ_NAN : v ? ve[k] : ke[k]);
+                const uint32_t c[2] = {code[k].x, code[k].y};
+                TO* o = reinterpret_cast<TO*>(&w);
+#pragma unroll
+                for (int x = 0; x < VEC / 4; ++x) {
+                    const uint32_t raw = kvq_raw<KIND>(c[x]), h0 = kvq_low<KIND>(raw), h1 = kvq_high<KIND>(raw);
+                    const float2 lo2 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), hi2 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                    o[4 * x] = il_from_f<TO>(lo2.x * f), o[4 * x + 1] = il_from_f<TO>(lo2.y * f);
+                    o[4 * x + 2] = il_from_f<TO>(hi2.x * f), o[4 * x + 3] = il_from_f<TO>(hi2.y * f);
+                }
+                if (told && v) w = make_uint4(0u, 0u, 0u, 0u);
+            }
+            *reinterpret_cast<uint4*>(out + (size_t)row * hd + d) = w;
+        }
     }
 }
 
 IL_EXPORT int il_kv_unpack(const void* cache, int kind, const int* block_table, int bt_stride, const int* entry_kvlen, const int* entry_qstart, int window,
-                           int first_entry, int n_entries, int width, int nkv, int hd, void* pages, int out_kind, int* table, int poison, cudaStream_t stream) {
+                           int first_entry, int n_entries, int width, int nkv, int hd, void* pages, int out_kind, int* table, int told_by_key, cudaStream_t stream) {
     const int n = n_entries - first_entry;
     if (n <= 0 || width <= 0) return IL_OK;
     if (hd > 256 || n > 65535) return IL_UNSUPPORTED;
     if (nkv <= 0 || hd <= 0 || hd % 16 || width > bt_stride || first_entry < 0 || (((uintptr_t)cache | (uintptr_t)pages) & 15)) return IL_BAD_ARG;
     if ((long long)n * width > 0x7fffffffLL) return IL_UNSUPPORTED;
     if ((kind != KVQ_E4M3 && kind != KVQ_INT8) || (out_kind != IL_F32 && out_kind != IL_BF16)) return IL_BAD_ARG;
-#define KVU_GO(TO, KIND)                                                                                                                                \
-    IL_LAUNCH((kv_unpack_kernel<TO, KIND>), dim3(width, n), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen, entry_qstart, \
-              window, first_entry, nkv, hd, (TO*)pages, table, poison)
+#define KVU_OF(TO, KIND, HD)                                                                                                                                \
+    IL_LAUNCH((kv_unpack_kernel<TO, KIND, HD>), dim3(width, n), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen, entry_qstart, \
+              window, first_entry, nkv, hd, (TO*)pages, table, told_by_key)
+#define KVU_GO(TO, KIND)                                 \
+    do {                                                 \
+        if (hd == 64) KVU_OF(TO, KIND, 64);              \
+        else if (hd == 128) KVU_OF(TO, KIND, 128);       \
+        else KVU_OF(TO, KIND, 0);                        \
+    } while (0)
     if (out_kind == IL_F32) {
         if (kind == KVQ_E4M3) KVU_GO(float, KVQ_E4M3);
         else KVU_GO(float, KVQ_INT8);
@@ -162,6 +339,7 @@ IL_EXPORT int il_kv_unpack(const void* cache, int kind, const int* block_table, 
         if (kind == KVQ_E4M3) KVU_GO(__nv_bfloat16, KVQ_E4M3);
         else KVU_GO(__nv_bfloat16, KVQ_INT8);
     }
+#undef KVU_OF
 #undef KVU_GO
     IL_LAUNCH_CHECK();
     return IL_OK;
