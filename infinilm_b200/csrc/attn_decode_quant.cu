@@ -628,9 +628,21 @@ IL_EXPORT int il_attn_decode_quant_resident_blocks(int group) {
 }
 
 // n_blocks: blocks that the pages are dealt out to, or 0: a block a unit. Scratch for n_blocks > 0: o_part float32 [2 * n_blocks * 16 * head_dim], ml_part [2 * n_blocks * 32].
-IL_EXPORT int il_attn_decode_quant(const void* q, long long q_stride, void* out, const void* cache, int kind, const int* block_table, int bt_stride,
-                                   const int* entry_kvlen, int n_decode, int nh, int nkv, int hd, float scale, int window, int n_blocks, float* o_part,
-                                   float* ml_part, int* status, int early, cudaStream_t stream) {
+// (Arguments as one struct: see kv_quant.cu.)
+struct DqArgs {
+    const void* q;
+    long long q_stride;
+    void* out;
+    const void* cache;
+    const int *block_table, *entry_kvlen;
+    float *o_part, *ml_part;
+    int* status;
+    cudaStream_t stream;
+    int kind, bt_stride, n_decode, nh, nkv, hd, window, n_blocks, early;
+    float scale;
+};
+IL_EXPORT int il_attn_decode_quant(const DqArgs* args) {
+    const auto [q, q_stride, out, cache, block_table, entry_kvlen, o_part, ml_part, status, stream, kind, bt_stride, n_decode, nh, nkv, hd, window, n_blocks, early, scale] = *args;
     if (n_decode <= 0) return IL_OK;
     if (hd != HEAD_DIM) return IL_UNSUPPORTED;
     if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !status) return IL_BAD_ARG;

@@ -84,6 +84,11 @@ class Workspace:
             self._bufs[key] = buf
         return buf[:n]
 
+    def address(self, tag: str, n: int, dtype: torch.dtype) -> int:
+        """Where a `flat` buffer of at least n elements lies, for a kernel's argument."""
+        buf = self._bufs.get((tag, "flat", dtype))
+        return buf.data_ptr() if buf is not None and buf.numel() >= n else self.flat(tag, n, dtype).data_ptr()
+
     def whole(self, tag: str, dtype: torch.dtype) -> torch.Tensor:
         """All of a `flat` buffer as it stands; replaced when a request for more replaces it."""
         return self._bufs[(tag, "flat", dtype)]

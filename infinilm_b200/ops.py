@@ -8,6 +8,7 @@ is not on a CUDA device, or a kernel library that cannot be built, raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import numpy as np
@@ -1833,30 +1834,55 @@ def kv_quant_record(head_dim: int) -> int:
     return 2 * KV_QUANT_PAGE * head_dim + 2 * KV_QUANT_PAGE
 
 
+# Arguments of the entry points below as the structs that they take (a ctypes call with twenty arguments of its own costs 3 us of host time, between kernels of a few microseconds).
+_STORE_ARGS, _UNPACK_ARGS, _DECODE_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<7Q10i"), struct.Struct("<Qq8Q9if")
+_quant_fns = {}
+
+
+def _quant_fn(name: str, lib: str, head_dim: int = 0):
+    """The entry point `name`, of the library for `head_dim` where there is one for each; looked up once."""
+    f = _quant_fns[name, head_dim] = _fn(lib, name, [ctypes.c_char_p], defines={"HEAD_DIM": head_dim} if head_dim else None)
+    return f
+
+
+def _packed(s: struct.Struct, what: str, *args) -> bytes:
+    try:
+        return s.pack(*args)
+    except struct.error as e:
+        raise KernelError(f"{what}: an argument out of range ({e})") from None
+
+
 def _quant_cache(what: str, cache: torch.Tensor, kind: str, n_kv_heads: int, head_dim: int) -> int:
     """The kind's number, the cache checked."""
     k = KV_KINDS.get(kind)
     if k is None:
         raise KernelError(f"{what}: the cache's kind is one of {', '.join(KV_KINDS)}, not {kind!r}")
-    if (cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[1] != n_kv_heads or cache.shape[2] != 32 * head_dim + 32
-            or not cache.is_contiguous()):
+    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[1:] != (n_kv_heads, 32 * head_dim + 32):
         raise KernelError(f"{what}: cache uint8 [pages, kv_heads, 32 * head_dim + 32], contiguous")
     return k
 
 
-def _on_one_device(what: str, *ts: Optional[torch.Tensor]) -> None:
-    """All on the current device, whose current stream the kernels are launched on."""
-    _need_cuda(*ts)
+def _on_one_device(what: str, *ts: torch.Tensor) -> int:
+    """All on the current device, whose current stream the kernels are launched on; its number."""
+    for t in ts:
+        if not t.is_cuda:
+            _need_cuda(t)
     d = _cur_device()
     for t in ts:
-        if t is not None and t.get_device() != d:
+        if t.get_device() != d:
             raise KernelError(f"{what}: a tensor on {t.device}; the kernels run on the current device, cuda:{d}")
+    return d
 
 
-def _descriptors(what: str, *ts: Optional[torch.Tensor]) -> None:
+def _descriptors(what: str, *ts: torch.Tensor) -> None:
     for t in ts:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t.dtype is not torch.int32 or not t.is_contiguous():
             raise KernelError(f"{what}: descriptors must be contiguous int32")
+
+
+def _status_ptr(d: int) -> int:
+    t = _stream_status.get(d)
+    return (t if t is not None else stream_status(torch.device("cuda", d))).data_ptr()
 
 
 def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tensor, tok_entry: torch.Tensor, block_table: torch.Tensor,
@@ -1866,26 +1892,29 @@ def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tens
     its columns of qkv itself, or memory of its own) and k and v as codes to their slots of the 8-bit cache (None: only q). qkv's columns of k and v are left
     as they are. Each token's slot is its own: what two rows write to one slot is undefined. A token whose block-table entry is below 0 is not stored.
     A row of k or v that is not finite is stored as NaN."""
-    T, what = qkv.shape[0], "rope_store_quant"
-    if qkv.dim() != 2 or q_out.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1:
+    what = "rope_store_quant"
+    nq = n_heads * head_dim
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != nq + 2 * n_kv_heads * head_dim:
         raise KernelError(f"{what}: qkv [T, (heads + 2 kv_heads) * head_dim], columns side by side")
-    if tuple(q_out.shape) != (T, n_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1:
+    T = qkv.shape[0]
+    if q_out.shape != (T, nq) or q_out.dtype is not qkv.dtype or q_out.stride(1) != 1:
         raise KernelError(f"{what}: q_out [T, heads * head_dim] of qkv's dtype, columns side by side")
     if T == 0:
         return
-    if q_out.stride(0) < n_heads * head_dim or qkv.stride(0) < qkv.shape[1]:
+    row, q_row = qkv.stride(0), q_out.stride(0)
+    if q_row < nq or row < nq:
         raise KernelError(f"{what}: rows must not overlap")
     _descriptors(what, tok_pos, tok_entry, block_table)
     if tok_pos.numel() != T or tok_entry.numel() != T or block_table.dim() != 2:
         raise KernelError(f"{what}: tok_pos and tok_entry int32 [T], block_table int32 [entries, width]")
-    if rot_dim and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rot_dim // 2 or not inv_freq.is_contiguous()):
+    if rot_dim and (inv_freq is None or inv_freq.dtype is not torch.float32 or inv_freq.numel() != rot_dim // 2 or not inv_freq.is_contiguous()):
         raise KernelError(f"{what}: inv_freq float32 [rot_dim / 2]")
     k = _quant_cache(what, cache, kind, n_kv_heads, head_dim) if cache is not None else KV_KINDS.get(kind, -1)
-    _on_one_device(what, qkv, q_out, tok_pos, tok_entry, block_table, cache, inv_freq)
-    f = _fn("kv_quant", "il_rope_store_quant", [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int,
-                                                _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_float, _c_void_p])
-    _check(f(_ptr(qkv), kind_of(qkv.dtype), qkv.stride(0), _ptr(q_out), q_out.stride(0), _ptr(tok_pos), _ptr(tok_entry), _ptr(block_table), block_table.shape[1],
-             _ptr(cache), k, T, n_heads, n_kv_heads, head_dim, rot_dim, _ptr(inv_freq if rot_dim else None), mscale, _stream()), what)
+    d = _on_one_device(what, qkv, q_out, tok_pos, tok_entry, block_table, *([cache] if cache is not None else []), *([inv_freq] if rot_dim else []))
+    f = _quant_fns.get(("il_rope_store_quant", 0)) or _quant_fn("il_rope_store_quant", "kv_quant")
+    _check(f(_packed(_STORE_ARGS, what, qkv.data_ptr(), row, q_out.data_ptr(), q_row, tok_pos.data_ptr(), tok_entry.data_ptr(), block_table.data_ptr(),
+                              0 if cache is None else cache.data_ptr(), inv_freq.data_ptr() if rot_dim else 0, _raw_stream(d), kind_of(qkv.dtype), block_table.shape[1], k, T,
+                              n_heads, n_kv_heads, head_dim, rot_dim, mscale)), what)
 
 
 def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_kvlen: torch.Tensor, pages: torch.Tensor,
@@ -1899,23 +1928,29 @@ def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_k
     `nan_in_keys`: for an attention that reads `pages` - a row of V that is NaN comes back as zeros and its row of K as NaN, so that
     who does not see the key does not get the NaN either."""
     what = "kv_unpack"
-    if pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[3] != KV_QUANT_PAGE or not pages.is_contiguous():
+    if pages.dim() != 5 or not pages.is_contiguous():
         raise KernelError(f"{what}: pages [entries * width, 2, kv_heads, 16, head_dim], contiguous")
-    n_kv_heads, head_dim = pages.shape[2], pages.shape[4]
+    room, two, n_kv_heads, slots, head_dim = pages.shape
+    if two != 2 or slots != KV_QUANT_PAGE:
+        raise KernelError(f"{what}: pages [entries * width, 2, kv_heads, 16, head_dim], contiguous")
     k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
-    _descriptors(what, block_table, entry_kvlen, table, entry_qstart)
+    _descriptors(what, block_table, entry_kvlen)
     if block_table.dim() != 2 or not 0 <= first_entry <= block_table.shape[0] or entry_kvlen.numel() < block_table.shape[0]:
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries], first_entry one of them")
     n_entries, width = block_table.shape
-    if entry_qstart is not None and entry_qstart.numel() < n_entries + 1:
-        raise KernelError(f"{what}: entry_qstart int32 [entries + 1]")
-    if pages.shape[0] < (n_entries - first_entry) * width or (table is not None and tuple(table.shape) != (n_entries, width)):
+    if entry_qstart is not None:
+        _descriptors(what, entry_qstart)
+        if entry_qstart.numel() < n_entries + 1:
+            raise KernelError(f"{what}: entry_qstart int32 [entries + 1]")
+    if table is not None:
+        _descriptors(what, table)
+    if room < (n_entries - first_entry) * width or (table is not None and table.shape != (n_entries, width)):
         raise KernelError(f"{what}: room for entries * width pages, table of the block table's shape")
-    _on_one_device(what, cache, block_table, entry_kvlen, pages, table, entry_qstart)
-    f = _fn("kv_quant", "il_kv_unpack", [_c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
-                                         _c_int, _c_void_p, _c_int, _c_void_p])
-    _check(f(_ptr(cache), k, _ptr(block_table), width, _ptr(entry_kvlen), _ptr(entry_qstart), int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
-             _ptr(pages), kind_of(pages.dtype), _ptr(table), int(nan_in_keys), _stream()), what)
+    d = _on_one_device(what, cache, block_table, entry_kvlen, pages, *(t for t in (table, entry_qstart) if t is not None))
+    f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
+    _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(), 0 if entry_qstart is None else entry_qstart.data_ptr(), pages.data_ptr(),
+                               0 if table is None else table.data_ptr(), _raw_stream(d), k, width, int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
+                               kind_of(pages.dtype), int(nan_in_keys))), what)
 
 
 _resident_quant = {}
@@ -1954,30 +1989,30 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     what = "attention_decode_quant"
     if n_decode <= 0:
         return
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1 or not out.is_contiguous():
+    nq = n_heads * head_dim
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1 or not out.is_contiguous():
         raise KernelError(f"{what}: bfloat16 q [rows, heads * head_dim] and contiguous out")
     if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise KernelError(f"{what}: head sizes {QUANT_HEAD_DIMS}, heads a multiple of kv_heads")
-    if q.shape[0] < n_decode or q.shape[1] < n_heads * head_dim or out.dim() != 2 or out.shape[0] < n_decode or out.shape[1] != n_heads * head_dim:
+    if out.dim() != 2 or out.shape[1] != nq or out.shape[0] < n_decode or q.shape[0] < n_decode or q.shape[1] < nq:
         raise KernelError(f"{what}: q [>= n_decode rows, >= heads * head_dim], out [>= n_decode rows, heads * head_dim]")
     k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
     _descriptors(what, block_table, entry_kvlen)
     if block_table.dim() != 2 or block_table.shape[0] < n_decode or entry_kvlen.numel() < n_decode:
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries]")
-    _on_one_device(what, q, out, cache, block_table, entry_kvlen)
-    w = int(window or 0)
-    seen = max(1, int(max_kvlen)) if not w else max(1, min(int(max_kvlen), abs(w) + KV_QUANT_PAGE))       # (a window may begin inside a page)
+    d = _on_one_device(what, q, out, cache, block_table, entry_kvlen)
+    w, seen = int(window or 0), int(max_kvlen)
+    if w:
+        seen = min(seen, abs(w) + KV_QUANT_PAGE)  # (a window may begin inside a page)
     group = n_heads // n_kv_heads
-    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE)
-    o_part = ml_part = None
-    if n_blocks > 0:
-        o_part, ml_part = ws.flat("quant_o_part", n_blocks * 32 * head_dim, torch.float32), ws.flat("quant_ml_part", n_blocks * 64, torch.float32)
-    f = _fn("attn_decode_quant", "il_attn_decode_quant", [_c_void_p, _c_ll, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int,
-                                                          _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p],
-            defines={"HEAD_DIM": head_dim})
-    _check(f(_ptr(q), q.stride(0), _ptr(out), _ptr(cache), k, _ptr(block_table), block_table.shape[1], _ptr(entry_kvlen), n_decode, n_heads, n_kv_heads, head_dim,
-             scale, w, n_blocks, _ptr(o_part), _ptr(ml_part), _ptr(stream_status(q.device)), int(cached_before), _stream()), what)
-    if n_blocks > 0:
+    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE))
+    parts = n_blocks > 0
+    f = _quant_fns.get(("il_attn_decode_quant", head_dim)) or _quant_fn("il_attn_decode_quant", "attn_decode_quant", head_dim)
+    _check(f(_packed(_DECODE_ARGS, what, q.data_ptr(), q.stride(0), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(),
+                               ws.address("quant_o_part", n_blocks * 32 * head_dim, torch.float32) if parts else 0,
+                               ws.address("quant_ml_part", n_blocks * 64, torch.float32) if parts else 0, _status_ptr(d), _raw_stream(d), k, block_table.shape[1], n_decode, n_heads,
+                               n_kv_heads, head_dim, w, n_blocks, int(cached_before), scale)), what)
+    if parts:
         count_launches(1)                         # the second kernel
 
 

@@ -99,6 +99,14 @@ def test_refused(call, kw, says):
         call(**kw)
 
 
+def test_numbers_that_do_not_fit_are_refused_too(monkeypatch):
+    monkeypatch.setattr(ops, "_on_one_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda d: 0)
+    monkeypatch.setattr(ops, "_quant_fn", lambda *a: (lambda args: 0))
+    with pytest.raises(ops.KernelError, match="out of range"):
+        _unpack(window=1 << 40)
+
+
 def test_nothing_to_do_is_no_call():
     _store(qkv=torch.zeros((0, (NH + 2 * NKV) * HD), dtype=BF), q_out=torch.zeros((0, NH * HD), dtype=BF))
     _decode(n_decode=0)
