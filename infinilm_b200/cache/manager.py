@@ -244,6 +244,8 @@ class CacheManager:
                 self.groups[g].entries.append(owner)
                 self.group_of_entry[owner] = g
         for g, grp in enumerate(self.groups):
+            if grp.need.quant is not None and self.kernel_page != self.KERNEL_PAGE:
+                raise ValueError(f"a cache of 8-bit codes takes pages of {self.KERNEL_PAGE} tokens or a multiple, not {self.page_size}")
             if grp.need.kind == "paged_kv":
                 grp.pool = PagePool((pages_per_group or {}).get(g, num_pages))
             elif grp.need.kind != "state":
@@ -265,6 +267,9 @@ class CacheManager:
                     # one page more than the pool hands out: padding rows of a replayed step write there
                     shape = ((grp.pool.n_pages + 1) * self.sub, 2, n.n_kv_heads, self.kernel_page, n.head_dim)
                     dt = self.dtype
+                    if n.quant is not None:       # a record of codes per page and kv head
+                        from .. import ops
+                        shape, dt = (shape[0], n.n_kv_heads, ops.kv_quant_record(n.head_dim)), torch.uint8
                 else:
                     # one slot more than are handed out: padding rows of a replayed step write there
                     shape = (self.slots.n_slots + 1,) + tuple(n.shape)
@@ -280,7 +285,9 @@ class CacheManager:
         b = 0
         for grp in self.groups:
             if grp.need.kind == "paged_kv":
-                b += len(grp.entries) * 2 * grp.need.n_kv_heads * grp.need.head_dim * elem_size
+                # (8-bit codes: a byte a number and one for the exponent of a row)
+                row = grp.need.head_dim * elem_size if grp.need.quant is None else grp.need.head_dim + 1
+                b += len(grp.entries) * 2 * grp.need.n_kv_heads * row
         return b
 
     # -- requests --------------------------------------------------------------------------
@@ -400,12 +407,13 @@ class CacheManager:
 @dataclass
 class PagedKVView:
     """What a mixer sees of a paged cache in one step."""
-    storage: object                               # [kernel pages, 2, kv_heads, page_size, head_dim]
+    storage: object                               # [kernel pages, 2, kv_heads, page_size, head_dim]; of 8-bit codes: uint8 [kernel pages, kv_heads, record]
     block_table: object                           # int32 [entries, width] on the device: kernel page ids
     page_size: int                                # tokens of a kernel page
     writable: bool = True
     max_pages: int = 0                            # width in use this step
     tma_map: object = None                        # tensor map of `storage` for kernels that copy pages by TMA
+    quant: Optional[str] = None                   # the kind of 8-bit codes that `storage` holds
 
 
 @dataclass

@@ -6,7 +6,7 @@ and the time.
     python -m infinilm_b200 --model DIR --enable-paged-attn --max-new-tokens 32 --prompt-len 64
     python -m infinilm_b200 --write-random-model DIR --config config.json --seed 0
 
-Options of other devices, parallelism, MoE, quantization, drafts and the server do not exist here.
+Options of other devices, parallelism, MoE, quantized weights, drafts and the server do not exist here.
 """
 from __future__ import annotations
 
@@ -48,6 +48,8 @@ def build_parser() -> argparse.ArgumentParser:
                    help="prefix reuse is not built; this flag is accepted and changes nothing")
     p.add_argument("--num-blocks", type=int, default=512, help="number of KV cache blocks")
     p.add_argument("--block-size", type=int, default=256, help="size of each KV cache block")
+    p.add_argument("--kv-cache-dtype", type=str, default="auto", choices=["auto", "fp8", "fp8_e4m3", "int8"],
+                   help="keep keys and values as 8-bit codes (fp8 e4m3 or whole numbers, a power of two per token and kv head); auto: in the compute dtype")
     p.add_argument("--skip-load", action="store_true", help="skip loading model weights (seeded random weights)")
     p.add_argument("--batch-size", type=int, default=1, help="copies of the prompt to generate for")
     p.add_argument("--max-batch-size", type=int, default=8, help="maximum number of live requests")
@@ -98,7 +100,7 @@ def main(argv=None) -> int:
               temperature=args.temperature, top_p=args.top_p, top_k=args.top_k, enable_graph=args.enable_graph,
               attn_backend=args.attn, skip_load=args.skip_load, enable_prefix_caching=False,
               max_num_batched_tokens=args.max_num_batched_tokens, chunk_size=args.chunk_size, seed=args.seed,
-              admission=args.admission)
+              admission=args.admission, kv_cache_dtype=args.kv_cache_dtype)
     sp = SamplingParams(temperature=args.temperature, top_p=args.top_p, top_k=args.top_k,
                         max_tokens=args.max_new_tokens, ignore_eos=args.ignore_eos)
     kw = {}
@@ -157,7 +159,8 @@ def bench_main(argv=None) -> int:
     llm = LLM(args.model, device=device, dtype=args.dtype, max_batch_size=max(args.max_batch_size, args.batch_size),
               max_tokens=max(outs), num_blocks=max(args.num_blocks, need_pages), block_size=args.block_size,
               enable_graph=args.enable_graph, attn_backend=args.attn, skip_load=args.skip_load,
-              max_num_batched_tokens=args.max_num_batched_tokens, chunk_size=args.chunk_size, seed=args.seed, admission=args.admission)
+              max_num_batched_tokens=args.max_num_batched_tokens, chunk_size=args.chunk_size, seed=args.seed, admission=args.admission,
+              kv_cache_dtype=args.kv_cache_dtype)
     results = []
     try:
         for n_in in ins:

@@ -37,6 +37,20 @@ def parse_dtype_name(name: str) -> str:
         raise ConfigError(f"unsupported dtype {name!r} (float32, float16, bfloat16)") from None
 
 
+# What a model's keys and values may be kept as: None (the compute dtype) or a kind of 8-bit codes.
+_KV_CACHE_NAMES = {"auto": None, "fp8": "fp8_e4m3", "fp8_e4m3": "fp8_e4m3", "int8": "int8"}
+
+
+def parse_kv_cache_dtype(name: Optional[str]) -> Optional[str]:
+    """Canonical name of a cache's kind, or None for the compute dtype (InfiniLM's option `--kv-cache-dtype`, `python/infinilm/base_config.py`, knows int8)."""
+    if name is None:
+        return None
+    try:
+        return _KV_CACHE_NAMES[str(name).lower()]
+    except KeyError:
+        raise ConfigError(f"unsupported kv_cache_dtype {name!r} ({', '.join(_KV_CACHE_NAMES)})") from None
+
+
 _REQUIRED = object()
 
 

@@ -16,9 +16,9 @@ import torch
 
 from .. import ops
 from ..cache.manager import CacheManager, SequenceCache
-from ..config.model_config import ModelConfig, parse_dtype_name
+from ..config.model_config import ModelConfig, parse_dtype_name, parse_kv_cache_dtype
 from ..config.registry import config_from_json, describe_model, load_config
-from ..models.causal_lm import CausalLM
+from ..models.causal_lm import CausalLM, quantise_caches
 from ..weights.loader import DictSource, FolderSource, TensorSource, load_into
 from .step import StepEntry, StepRunner
 
@@ -28,9 +28,10 @@ _TORCH_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16}
 class Engine:
     def __init__(self, config: ModelConfig, source: TensorSource, dtype: str = "bfloat16", device: str = "cuda:0",
                  page_size: int = 16, num_pages: Optional[int] = None, max_tokens: Optional[int] = None,
-                 max_seqs: int = 64, max_batch_tokens: int = 8192, progress=None):
+                 max_seqs: int = 64, max_batch_tokens: int = 8192, progress=None, kv_cache_dtype: Optional[str] = None):
         """`num_pages` pages of `page_size` tokens per cache group, or enough for `max_tokens`
-        cached tokens (each request's count rounded up to whole pages)."""
+        cached tokens (each request's count rounded up to whole pages). `kv_cache_dtype`: "fp8_e4m3" or "int8" - keys and values are kept as 8-bit
+        codes with a power of two per token and kv head (pages of 16 tokens or a multiple; models of plain grouped-query attention); None or "auto": in the compute dtype."""
         if not torch.cuda.is_available():
             raise RuntimeError("infinilm_b200 runs on a CUDA device (sm_100a); none is visible and there is no CPU path")
         name = parse_dtype_name(dtype)
@@ -41,7 +42,10 @@ class Engine:
         torch.cuda.set_device(self.device)
         # Library matrix products never use a reduced-precision mode on the float32 path.
         torch.backends.cuda.matmul.allow_tf32 = False
-        self.model = CausalLM(describe_model(config), self.dtype)
+        self.kv_cache_dtype = parse_kv_cache_dtype(kv_cache_dtype)
+        spec = describe_model(config)
+        quantise_caches(spec, self.kv_cache_dtype)
+        self.model = CausalLM(spec, self.dtype)
         load_into(self.model, source, self.device, progress)
         if num_pages is None:
             if max_tokens is None:

@@ -467,7 +467,7 @@ class StepRunner:
                 grp = groups[g]
                 if grp.need.kind == "paged_kv":
                     return PagedKVView(grp.storage[owner], view(s_bt[g]).view(Ep, widths[g]), kpage,
-                                       writable=writable, max_pages=widths[g], tma_map=grp.tma_maps.get(owner))
+                                       writable=writable, max_pages=widths[g], tma_map=grp.tma_maps.get(owner), quant=grp.need.quant)
                 return StateView(grp.storage[owner], view(s_rs), view(s_wsl), writable=writable)
 
             for i, owner in enumerate(owners):

@@ -52,11 +52,12 @@ class LLM:
                  temperature: float = 1.0, top_p: float = 0.8, top_k: int = 1, enable_graph: bool = False,
                  attn_backend: str = "default", skip_load: bool = False, enable_prefix_caching: bool = False,
                  max_num_batched_tokens: Optional[int] = None, chunk_size: int = 2048, seed: int = 0,
-                 admission: str = "worst_case", pipelined: bool = True, _config: Optional[ModelConfig] = None,
+                 admission: str = "worst_case", pipelined: bool = True, kv_cache_dtype: Optional[str] = None, _config: Optional[ModelConfig] = None,
                  _tensors: Optional[Mapping[str, torch.Tensor]] = None):
         """`model_path`: folder with config.json and safetensors. `skip_load`: random weights
         (seeded) instead of the folder's. `num_blocks` pages of `block_size` tokens. `pipelined`: a
-        step's tokens are read back while the next step runs (the next step gets them on the device)."""
+        step's tokens are read back while the next step runs (the next step gets them on the device). `kv_cache_dtype`: "fp8_e4m3" (or "fp8") or "int8" keeps
+        keys and values as 8-bit codes, in half the memory; "auto" or None in the compute dtype."""
         if tensor_parallel_size != 1 or pipeline_parallel_size != 1:
             raise ValueError("this engine runs on one GPU: tensor_parallel_size and pipeline_parallel_size must be 1")
         if cache_type != "paged":
@@ -75,7 +76,7 @@ class LLM:
             dtype = "bfloat16"                    # 16-bit weights are kept as bfloat16
         mnbt = max_num_batched_tokens or int(os.environ.get("INFINILM_MAX_NUM_BATCHED_TOKENS", "0")) or 8192
         kw = dict(dtype=dtype, device=dev, page_size=block_size, num_pages=num_blocks, max_seqs=max_batch_size,
-                  max_batch_tokens=mnbt)
+                  max_batch_tokens=mnbt, kv_cache_dtype=kv_cache_dtype)
         if _tensors is not None:
             self.engine = Engine.from_tensors(cfg, _tensors, **kw)
         elif skip_load:

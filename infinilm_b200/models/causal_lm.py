@@ -12,8 +12,19 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from .. import ops
+from ..config.model_config import ConfigError
 from ..parts.base import Part, build_part, part_class
 from ..parts.spec import CacheNeed, ModelSpec, WeightSpec
+
+
+def quantise_caches(spec: ModelSpec, kind: Optional[str]) -> None:
+    """Has every layer of `spec` keep its keys and values as 8-bit codes of `kind` (None: nothing to do); a layer whose mixer has no such cache is an error."""
+    if kind is None:
+        return
+    for i, ls in enumerate(spec.layers):
+        if not part_class("mixer", ls.mixer.kind).takes_quant_cache:
+            raise ConfigError(f"kv_cache_dtype {kind}: the cache of layer {i}'s mixer ({ls.mixer.kind}) has no 8-bit form")
+        ls.mixer.params["kv_cache"] = kind
 
 
 class CausalLM:

@@ -8,6 +8,7 @@ ranges of one weight).
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 import os
 import warnings
@@ -83,7 +84,30 @@ class PagedAttend:
         target = max(1, int(resident * self.WAVE_FILL))
         return max(1, min(target // base, (max_pages + 3) // 4, 128))
 
+    def run_quant(self, qkv, out, ctx, cache) -> None:
+        """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and `run` attends over those."""
+        n_dec, E = ctx.n_decode, ctx.n_entries
+        fast = (self.dtype == torch.bfloat16 and not self.force_plain and self.hd in ops.QUANT_HEAD_DIMS and self.sink is None and self.dist_bias is None
+                and not self.sigmoid and self.cap is None)
+        if fast and n_dec > 0:
+            ops.attention_decode_quant(qkv, out, cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, n_dec, self.nh, self.nkv, self.hd, self.scale,
+                                       self.mask_arg, max(ctx.h_kvlen[:n_dec]), ctx.ws, cached_before=True)
+        if fast and E == n_dec:
+            return
+        if fast and self.prefill_kernel != "mma" and ops.prefill_tc5_ok(self.hd, self.nh // self.nkv, cache.page_size):
+            per = ops.prefill_quant_tokens(self.nh, self.nkv, self.hd)
+            ops.attention_prefill_quant(qkv, out, cache.storage, cache.quant, cache.block_table, ctx.entry_qstart, ctx.entry_kvlen, n_dec, E, ctx.prompt_tiles(per),
+                                        self.nh, self.nkv, self.hd, self.scale, self.mask_arg, ctx.ws, n_tiles_rule=(qkv.shape[0] - n_dec + per - 1) // per + E - n_dec - 1)
+            return
+        width = cache.block_table.shape[1]
+        pages, tma_map = ops.unpacked_cache(ctx.ws, E * width, self.nkv, self.hd, self.dtype)
+        table = ctx.ws.flat("kv_unpacked_table", E * width, torch.int32).view(E, width)
+        ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, nan_in_keys=True)
+        self.run(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None))
+
     def run(self, qkv, out, ctx, cache) -> None:
+        if getattr(cache, "quant", None) is not None:
+            return self.run_quant(qkv, out, ctx, cache)
         G = self.nh // self.nkv
         if not self.fast_ok(cache.page_size):
             if self.dtype == torch.bfloat16 and not self.force_plain and not PagedAttend._warned_plain:
@@ -133,7 +157,9 @@ class PagedAttend:
 
 class Attention(Mixer):
     """params: hidden, n_heads, n_kv_heads, head_dim, qkv_bias, out_bias, out_scale,
-    window (None = all keys), position (PartSpec of a position encoding)."""
+    window (None = all keys), position (PartSpec of a position encoding), kv_cache (None, or the kind of 8-bit codes that keys and values are kept as)."""
+
+    takes_quant_cache = True
 
     def __init__(self, params, prefix, dtype):
         super().__init__(params, prefix, dtype)
@@ -148,6 +174,9 @@ class Attention(Mixer):
         self.force_plain = bool(p.get("plain_kernel", False))
         self.prefill_kernel = str(p.get("prefill_kernel", os.environ.get("INFINILM_B200_PREFILL_ATTN", "auto")))   # "mma": never tcgen05
         self.fuse_rope = os.environ.get("INFINILM_B200_FUSE_ROPE", "1") != "0"
+        self.kv_cache: Optional[str] = p.get("kv_cache")
+        if self.kv_cache is not None and self.kv_cache not in ops.KV_KINDS:
+            raise ValueError(f"attention: kv_cache is one of {', '.join(ops.KV_KINDS)}, not {self.kv_cache!r}")
         self.scale = 1.0 / math.sqrt(self.hd)
         self.core = PagedAttend(dtype, self.nh, self.nkv, self.hd, self.scale, self.window, self.force_plain, self.prefill_kernel)
         self.n_qkv = (self.nh + 2 * self.nkv) * self.hd
@@ -183,13 +212,15 @@ class Attention(Mixer):
         self.position.to_device(w.device)
 
     def cache_need(self) -> Optional[CacheNeed]:
-        return CacheNeed("paged_kv", n_kv_heads=self.nkv, head_dim=self.hd, window=self.window)
+        return CacheNeed("paged_kv", n_kv_heads=self.nkv, head_dim=self.hd, window=self.window, quant=self.kv_cache)
 
     @property
     def graph_safe(self):
         return self.position.graph_safe or not self.position.has_transform
 
     def accepts_normed(self, T):
+        if self.kv_cache is not None:             # a row's exponent needs the whole head: rotation and codes are a kernel of their own behind the projection
+            return self.dtype == torch.bfloat16 and ops.skinny_ok(T, self.hidden)
         return (self.dtype == torch.bfloat16 and self.fuse_rope and not self.position.has_transform
                 and ops.skinny_rope_ok(T, self.hidden, self.hd, self.position.rot_dim))
 
@@ -201,6 +232,16 @@ class Attention(Mixer):
         pos = self.position
         qkv = ctx.ws.rows("qkv", T, self.n_qkv, self.dtype)
         store = cache.storage if cache.writable else None
+        if self.kv_cache is not None:
+            if isinstance(x, ops.NormedInput):
+                ops.gemm_skinny(x.xw, self.qkv.weight, qkv, self.qkv.alpha, self.qkv.bias, norm_in=x, w_static=True)
+            else:
+                self.qkv(x, qkv)
+            if pos.has_transform:
+                pos.transform(qkv, ctx, self.nh, self.nkv, self.hd)
+            ops.rope_store_quant(qkv, qkv[:, :self.nh * self.hd], ctx.tok_pos, ctx.tok_entry, cache.block_table, store, self.kv_cache, self.nh, self.nkv, self.hd,
+                                 pos.rot_dim, pos.inv_freq, pos.mscale)
+            return self._attend_and_project(qkv, ctx, cache, tail)
         if (self.dtype == torch.bfloat16 and self.fuse_rope and not pos.has_transform
                 and ops.skinny_rope_ok(T, self.hidden, self.hd, pos.rot_dim)):
             # a few rows (decode): the projection rotates q and k and writes k, v to the cache in its epilogue
@@ -214,6 +255,10 @@ class Attention(Mixer):
                 pos.transform(qkv, ctx, self.nh, self.nkv, self.hd)
             ops.rope_store(qkv, ctx.tok_pos, ctx.tok_entry, cache.block_table, store, cache.page_size,
                            self.nh, self.nkv, self.hd, pos.rot_dim, pos.inv_freq, pos.mscale)
+        return self._attend_and_project(qkv, ctx, cache, tail)
+
+    def _attend_and_project(self, qkv, ctx, cache, tail):
+        T = qkv.shape[0]
         out = ctx.ws.rows("attn_out", T, self.nh * self.hd, self.dtype)
         self.attend(qkv, out, ctx, cache)
         if tail is not None:                      # o_proj adds into the residual and prepares the next norm itself

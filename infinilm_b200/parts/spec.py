@@ -98,6 +98,7 @@ class CacheNeed:
     window: Optional[int] = None
     shape: Tuple[int, ...] = ()
     dtype: str = "compute"                      # "compute" | "float32" | "int32"
+    quant: Optional[str] = None                 # paged_kv: the kind of 8-bit codes that keys and values are kept as
 
     def group_key(self) -> Tuple:
-        return (self.kind, self.n_kv_heads, self.head_dim, self.window, tuple(self.shape), self.dtype)
+        return (self.kind, self.n_kv_heads, self.head_dim, self.window, tuple(self.shape), self.dtype, self.quant)

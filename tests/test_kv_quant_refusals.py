@@ -115,3 +115,44 @@ def test_nothing_to_do_is_no_call():
 
 def test_record_bytes():
     assert ops.kv_quant_record(128) == 4128 and ops.kv_quant_record(64) == 2080
+
+
+# ---- configuration ---
+def test_names_of_the_option():
+    from infinilm_b200.cli import build_parser
+    from infinilm_b200.config.model_config import ConfigError, parse_kv_cache_dtype
+    assert [parse_kv_cache_dtype(n) for n in (None, "auto", "fp8", "fp8_e4m3", "INT8")] == [None, None, "fp8_e4m3", "fp8_e4m3", "int8"]
+    with pytest.raises(ConfigError, match="kv_cache_dtype 'int4'"):
+        parse_kv_cache_dtype("int4")
+    assert build_parser().parse_args([]).kv_cache_dtype == "auto"
+    assert build_parser().parse_args(["--kv-cache-dtype", "int8"]).kv_cache_dtype == "int8"
+    with pytest.raises(SystemExit):
+        build_parser().parse_args(["--kv-cache-dtype", "bf16"])
+
+
+def test_a_model_whose_layers_have_no_such_cache_is_refused():
+    from tiny_configs import tiny_b
+
+    import gopitar_configs
+    from infinilm_b200.config.model_config import ConfigError
+    from infinilm_b200.config.registry import config_from_json, describe_model
+    from infinilm_b200.models.causal_lm import CausalLM, quantise_caches
+    spec = describe_model(config_from_json(tiny_b()))
+    quantise_caches(spec, "int8")
+    assert all(n.quant == "int8" for n in CausalLM(spec, torch.bfloat16).cache_needs())
+    raw = gopitar_configs.gp_a()
+    with pytest.raises(ConfigError, match="no 8-bit form"):
+        quantise_caches(describe_model(config_from_json(raw)), "int8")
+    with pytest.raises(ValueError, match="kv_cache is one of"):
+        spec.layers[0].mixer.params["kv_cache"] = "int4"
+        CausalLM(spec, torch.bfloat16)
+
+
+def test_pages_of_such_a_cache():
+    from infinilm_b200.cache.manager import CacheManager
+    from infinilm_b200.parts.spec import CacheNeed
+    need = CacheNeed("paged_kv", n_kv_heads=2, head_dim=64, quant="int8")
+    cm = CacheManager([need, CacheNeed("paged_kv", n_kv_heads=2, head_dim=64)], 32, 4, 2)
+    assert len(cm.groups) == 2 and cm.bytes_per_token(2) == 2 * (2 * 64 + 2) + 2 * 2 * 64 * 2
+    with pytest.raises(ValueError, match="pages of 16"):
+        CacheManager([need], 8, 4, 2)
