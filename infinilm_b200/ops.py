@@ -767,6 +767,19 @@ def _has_third_map(kv_map: torch.Tensor) -> bool:
     return ok
 
 
+_prefill_tc5_fns = {}
+
+
+def _prefill_tc5_fn(head_dim: int):
+    f = _prefill_tc5_fns.get(head_dim)
+    if f is None:
+        f = _prefill_tc5_fns[head_dim] = _fn(
+            "attn_prefill_tc5", "il_attn_prefill_tc5",
+            [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+             _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_float, _c_void_p], defines={"HEAD_DIM": head_dim})
+    return f
+
+
 def attention_prefill_tc5(qkv: torch.Tensor, out: torch.Tensor, kv_map: torch.Tensor, block_table: torch.Tensor,
                           entry_qstart: torch.Tensor, entry_kvlen: torch.Tensor, first_entry: int, n_entries: int,
                           n_tiles_total: int, page_size: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
@@ -792,10 +805,7 @@ def attention_prefill_tc5(qkv: torch.Tensor, out: torch.Tensor, kv_map: torch.Te
     if out.shape != (qkv.shape[0], n_heads * head_dim):
         raise KernelError("attention_prefill_tc5: out [T, heads*head_dim]")
     _contig("qkv", qkv), _contig("out", out), _contig("block_table", block_table)
-    f = _fn("attn_prefill_tc5", "il_attn_prefill_tc5",
-            [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
-             _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_float, _c_void_p], defines={"HEAD_DIM": head_dim})
-    _check(f(_ptr(qkv), qkv.shape[1], _ptr(out), _c_void_p(kv_map.data_ptr() + 256), _ptr(block_table), block_table.shape[1],
+    _check(_prefill_tc5_fn(head_dim)(_ptr(qkv), qkv.shape[1], _ptr(out), _c_void_p(kv_map.data_ptr() + 256), _ptr(block_table), block_table.shape[1],
              _ptr(entry_qstart), _ptr(entry_kvlen), page_size, first_entry, n_entries, n_tiles_total,
              n_tiles_total if n_tiles_rule is None else n_tiles_rule, n_heads, n_kv_heads, head_dim, scale, int(window or 0), _ptr(stream_status(qkv.device)), _ptr(sink), _ptr(dist_bias), 0 if dist_bias is None else dist_bias.shape[0] - 1,
              int(sigmoid), _ptr(log_bias), cap, _stream()), "attention_prefill_tc5")
@@ -2024,12 +2034,19 @@ def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
 def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype):
     """A workspace's pages for `kv_unpack` ([n_pages, 2, kv_heads, 16, head_dim]) and, for bfloat16, their tensor map (see `kv_tensor_map`; None where there is none)."""
     per = 2 * n_kv_heads * KV_QUANT_PAGE * head_dim
-    flat = ws.flat("kv_unpacked", n_pages * per, dtype)
-    whole, kept = ws.whole("kv_unpacked", dtype), ws.kept.get(("kv_unpacked", n_kv_heads, head_dim, dtype))
-    if kept is None or kept[0] is not whole:      # (a buffer that grew is another one)
+    kv_map = _unpacked_map(ws, n_pages, n_kv_heads, head_dim) if dtype is torch.bfloat16 else None
+    return ws.flat("kv_unpacked", n_pages * per, dtype).view(n_pages, 2, n_kv_heads, KV_QUANT_PAGE, head_dim), kv_map
+
+
+def _unpacked_map(ws, n_pages: int, n_kv_heads: int, head_dim: int) -> Optional[torch.Tensor]:
+    """The tensor map of a workspace's bfloat16 pages, of which there are n_pages at least; kept beside the buffer (one that grew is another one)."""
+    per = 2 * n_kv_heads * KV_QUANT_PAGE * head_dim
+    ws.address("kv_unpacked", n_pages * per, torch.bfloat16)
+    whole, kept = ws.whole("kv_unpacked", torch.bfloat16), ws.kept.get(("kv_unpacked", n_kv_heads, head_dim))
+    if kept is None or kept[0] is not whole:
         full = whole[:whole.numel() // per * per].view(-1, 2, n_kv_heads, KV_QUANT_PAGE, head_dim)
-        kept = ws.kept[("kv_unpacked", n_kv_heads, head_dim, dtype)] = (whole, kv_tensor_map(full) if dtype == torch.bfloat16 else None)
-    return flat.view(n_pages, 2, n_kv_heads, KV_QUANT_PAGE, head_dim), kept[1]
+        kept = ws.kept["kv_unpacked", n_kv_heads, head_dim] = (whole, kv_tensor_map(full))
+    return kept[1]
 
 
 def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_qstart: torch.Tensor,
@@ -2043,20 +2060,28 @@ def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Ten
     what = "attention_prefill_quant"
     if n_entries <= first_entry or n_tiles_total <= 0:
         return
-    if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads or not prefill_tc5_ok(head_dim, n_heads // n_kv_heads, KV_QUANT_PAGE):
+    nq = n_heads * head_dim
+    if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads // n_kv_heads > 128:
         raise KernelError(f"{what}: head sizes {QUANT_HEAD_DIMS}, heads a multiple of kv_heads and at most 128 of them")
-    if q.dim() != 2 or q.shape[1] < n_heads * head_dim or block_table.dim() != 2 or block_table.shape[0] < n_entries or first_entry < 0:
-        raise KernelError(f"{what}: q [T, >= heads * head_dim], block_table int32 [entries, width]")
-    if entry_qstart.numel() < n_entries + 1 or entry_kvlen.numel() < n_entries:
-        raise KernelError(f"{what}: entry_qstart int32 [entries + 1], entry_kvlen int32 [entries]")
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or q.dim() != 2 or not q.is_contiguous() or q.shape[1] < nq:
+        raise KernelError(f"{what}: bfloat16 q [T, >= heads * head_dim], contiguous")
+    if not out.is_contiguous() or out.shape != (q.shape[0], nq):
+        raise KernelError(f"{what}: out bfloat16 [T, heads * head_dim], contiguous")
+    k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
     _descriptors(what, block_table, entry_qstart, entry_kvlen)
-    _on_one_device(what, q, out, cache, block_table, entry_qstart, entry_kvlen)
-    block_table = block_table[:n_entries]
-    width = block_table.shape[1]
-    pages, kv_map = unpacked_cache(ws, (n_entries - first_entry) * width, n_kv_heads, head_dim, torch.bfloat16)
-    if kv_map is None:
+    if block_table.dim() != 2 or first_entry < 0 or block_table.shape[0] < n_entries or entry_qstart.numel() < n_entries + 1 or entry_kvlen.numel() < n_entries:
+        raise KernelError(f"{what}: block_table int32 [entries, width], entry_qstart int32 [entries + 1], entry_kvlen int32 [entries], first_entry one of them")
+    d = _on_one_device(what, q, out, cache, block_table, entry_qstart, entry_kvlen)
+    width, w, stream = block_table.shape[1], int(window or 0), _raw_stream(d)
+    n_pages = (n_entries - first_entry) * width
+    kv_map = _unpacked_map(ws, n_pages, n_kv_heads, head_dim)
+    if kv_map is None or not _has_third_map(kv_map):
         raise KernelError(f"{what}: the driver has no tensor map for this cache")
-    table = ws.flat("kv_unpacked_table", n_entries * width, torch.int32).view(n_entries, width)
-    kv_unpack(cache, kind, block_table, entry_kvlen, pages, table, entry_qstart, window, first_entry, nan_in_keys=True)
-    attention_prefill_tc5(q, out, kv_map, table, entry_qstart, entry_kvlen, first_entry, n_entries, n_tiles_total, KV_QUANT_PAGE, n_heads, n_kv_heads, head_dim,
-                          scale, window, n_tiles_rule=n_tiles_rule)
+    table = ws.address("kv_unpacked_table", n_entries * width, torch.int32)
+    qstart, kvlen = entry_qstart.data_ptr(), entry_kvlen.data_ptr()
+    f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
+    _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), kvlen, qstart, ws.address("kv_unpacked", n_pages * 32 * n_kv_heads * head_dim, torch.bfloat16),
+                     table, stream, k, width, w, first_entry, n_entries, width, n_kv_heads, head_dim, BF16, 1)), what)
+    _check(_prefill_tc5_fn(head_dim)(q.data_ptr(), q.shape[1], out.data_ptr(), kv_map.data_ptr() + 256, table, width, qstart, kvlen, KV_QUANT_PAGE, first_entry, n_entries, n_tiles_total,
+                                     n_tiles_total if n_tiles_rule is None else n_tiles_rule, n_heads, n_kv_heads, head_dim, scale, w, _status_ptr(d), None, None, 0, 0, None, 0.0, stream),
+           what)

@@ -89,7 +89,9 @@ CASES = [
     (_prefill, dict(q=torch.zeros((T, NH * HD - 8), dtype=BF)), "q "),
     (_prefill, dict(entry_qstart=_i(2)), "entry_qstart"),
     (_prefill, dict(block_table=_i(1, 2)), "block_table"),
-    (_prefill, dict(first_entry=-1), "q "),
+    (_prefill, dict(first_entry=-1), "first_entry"),
+    (_prefill, dict(out=torch.zeros((T + 1, NH * HD), dtype=BF)), "out"),
+    (_prefill, dict(kind="fp4"), "kind is one of"),
 ]
 
 
