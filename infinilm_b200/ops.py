@@ -1026,7 +1026,7 @@ def stream_status(device) -> torch.Tensor:
 
 # What a kernel whose bounded wait ran out leaves in its stream's status word: from, to, the kernel's file.
 STATUS_CODES = ((11, 14, "gemm_tc5"), (21, 21, "attn_decode"), (30, 39, "attn_prefill_tc5"), (51, 54, "gemm_mid"), (71, 75, "gemm_f32"),
-                (81, 83, "gemm_narrow_tc5"), (91, 91, "attn_decode_quant"))
+                (81, 83, "gemm_narrow_tc5"), (91, 91, "attn_decode_quant"), (101, 109, "attn_prefill_pair"))
 
 
 def check_status(device) -> None:
@@ -1845,7 +1845,8 @@ def kv_quant_record(head_dim: int) -> int:
 
 
 # Arguments of the entry points below as the structs that they take (a ctypes call with twenty arguments of its own costs 3 us of host time, between kernels of a few microseconds).
-_STORE_ARGS, _UNPACK_ARGS, _DECODE_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<7Q10i"), struct.Struct("<Qq8Q9if")
+_STORE_ARGS, _UNPACK_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<7Q10i")
+_DECODE_ARGS, _PAIR_ARGS = struct.Struct("<Qq8Q9if"), struct.Struct("<Qq7Q8if")
 _quant_fns = {}
 
 
@@ -2026,9 +2027,16 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
         count_launches(1)                         # the second kernel
 
 
+# Blocks (pairs of row tiles x kv heads) from which on prompts take the kernel with two row tiles a block; fewer take the one with half of that a block, which also shares long chains
+# among blocks. One row tile / two, us: 1,024 tokens of 32 heads on 2 of 128 (128 blocks) 27.3 / 27.6, 1,536 (192) 38.5 / 36.4, 2,048 (256) 53.7 / 50.8; four prompts of 300, 32 on 8 (160),
+# 26.8 / 32.0; 512 tokens behind 4,096 (64) 56 / 76; eight times 200 behind 4,000 (208) 157 / 147; 2,048 tokens of 16 heads on 2 of 64 (128) 35.1 / 35.4, 4,096 (256) 76.8 / 61.7.
+PAIR_FROM = 192
+
+
 def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     """Consecutive tokens of a request that one block of `attention_prefill_quant` takes: its tiles are counted by this."""
-    return max(1, prefill_tc5_rows(head_dim) // (n_heads // n_kv_heads))
+    group = n_heads // n_kv_heads
+    return 2 * max(1, 128 // group) if head_dim <= 128 else max(1, prefill_tc5_rows(head_dim) // group)
 
 
 def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype):
@@ -2082,6 +2090,14 @@ def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Ten
     f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
     _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), kvlen, qstart, ws.address("kv_unpacked", n_pages * 32 * n_kv_heads * head_dim, torch.bfloat16),
                      table, stream, k, width, w, first_entry, n_entries, width, n_kv_heads, head_dim, BF16, 1)), what)
+    rule = n_tiles_total if n_tiles_rule is None else n_tiles_rule
+    if head_dim <= 128 and rule * n_kv_heads >= PAIR_FROM:
+        f = _quant_fns.get(("il_attn_prefill_pair", head_dim)) or _quant_fn("il_attn_prefill_pair", "attn_prefill_pair", head_dim)
+        _check(f(_packed(_PAIR_ARGS, what, q.data_ptr(), q.shape[1], out.data_ptr(), kv_map.data_ptr() + 256, table, qstart, kvlen, _status_ptr(d), stream, width, first_entry,
+                         n_entries, n_tiles_total, n_heads, n_kv_heads, head_dim, w, scale)), what)
+        return
+    if head_dim <= 128:                           # (tiles of half as many tokens: at most twice as many of them, and blocks without tokens leave at once)
+        n_tiles_total, rule = 2 * n_tiles_total, 2 * rule
     _check(_prefill_tc5_fn(head_dim)(q.data_ptr(), q.shape[1], out.data_ptr(), kv_map.data_ptr() + 256, table, width, qstart, kvlen, KV_QUANT_PAGE, first_entry, n_entries, n_tiles_total,
-                                     n_tiles_total if n_tiles_rule is None else n_tiles_rule, n_heads, n_kv_heads, head_dim, scale, w, _status_ptr(d), None, None, 0, 0, None, 0.0, stream),
+                                     rule, n_heads, n_kv_heads, head_dim, scale, w, _status_ptr(d), None, None, 0, 0, None, 0.0, stream),
            what)

@@ -367,8 +367,11 @@ def test_offsets_past_32_bits(cuda_device):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 64), (4, 4, 128), (32, 2, 128), (4, 1, 256), (6, 2, 64)])
 @pytest.mark.parametrize("window", [None, 40, -32])
-def test_prompt_portions_over_codes(cuda_device, kind, nh, nkv, hd, window):
+@pytest.mark.parametrize("pair_from", [0, 1 << 30])
+def test_prompt_portions_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, window, pair_from):
+    """With two row tiles a block and with one."""
     ops, dev = _ops(), cuda_device
+    monkeypatch.setattr(ops, "PAIR_FROM", pair_from)
     cached, new = [9, 0, 100, 0, 31], [1, 37, 20, 1, 80]     # the first entry is a single token that another kernel takes
     kvlens = [a + b for a, b in zip(cached, new)]
     rows, n_pages = _tables(kvlens, 2, 12)
@@ -397,6 +400,48 @@ def test_prompt_portions_over_codes(cuda_device, kind, nh, nkv, hd, window):
                 assert torch.isnan(row[:nh // nkv]).all()
                 row, want, mag = row[nh // nkv:], want[nh // nkv:], mag[nh // nkv:]
             # the output's rounding, the weights' to bfloat16 (both 2^-8), the rest in 32 bits
+            room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -8 + 2.0 ** -14)
+            assert ((row - want).abs() <= room).all(), (e, i, ((row - want).abs() / room.clamp(min=1e-300)).max())
+    ops.check_status(dev)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 64), (8, 1, 128), (3, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("pair_from", [0, 1 << 30])
+def test_long_portions_with_many_key_tiles(cuda_device, monkeypatch, kind, nh, nkv, hd, window, pair_from):
+    """Chains of key tiles, rows of a block's two halves with chains of unequal length, large scores (the running maximum is raised tile after tile), a NaN that late tokens see."""
+    ops, dev = _ops(), cuda_device
+    monkeypatch.setattr(ops, "PAIR_FROM", pair_from)
+    cached, new = [700, 0, 1111], [900, 129, 3]
+    kvlens = [a + b for a, b in zip(cached, new)]
+    rows, n_pages = _tables(kvlens, 2, 30)
+    g = torch.Generator().manual_seed(31)
+    kv = torch.randn((n_pages, nkv, 2, 16, hd), generator=g)
+    for e, n in enumerate(kvlens):                # keys grow along the request
+        for p in range((n + 15) // 16):
+            kv[rows[e][p], :, 0] *= 0.2 + 3.0 * p * 16 / max(kvlens)
+    rec = P.make_records(kv, kind)
+    val = P.decode_records(rec, hd, kind)
+    rec[rows[0][90], 0, 32 * hd + 5] = 255        # key 1445 of the first request
+    T, qs = sum(new), [0, 900, 1029, 1032]
+    q = torch.randn((T, nh * hd), generator=g).to(torch.bfloat16)
+    per, scale = ops.prefill_quant_tokens(nh, nkv, hd), 1.0 / math.sqrt(hd)
+    out = torch.full((T, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
+    args = (rec.to(dev), kind, _i32(rows, dev), _i32(qs, dev), _i32(kvlens, dev), 0, 3, sum((n + per - 1) // per for n in new), nh, nkv, hd, scale, window)
+    ops.attention_prefill_quant(q.to(dev), out, *args, _ws(dev))
+    again = torch.empty_like(out)
+    ops.attention_prefill_quant(q.to(dev), again, *args, _ws(dev))
+    assert torch.equal(out.nan_to_num(nan=7.0), again.nan_to_num(nan=7.0))
+    got = out.cpu().double()
+    for e in range(3):
+        for i in sorted({0, 1, new[e] - 1, new[e] // 2, *range(3, new[e], 41)}):
+            pos, t = cached[e] + i, qs[e] + i
+            row = got[t].view(nh, hd)
+            if e == 0 and P.mask_lo(pos, window or 0) <= 1445 <= pos:
+                assert torch.isnan(row[:nh // nkv]).all()
+                continue
+            want, mag = P.attend(q[t].view(nh, hd), val, rows[e], pos, scale, window or 0)
             room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -8 + 2.0 ** -14)
             assert ((row - want).abs() <= room).all(), (e, i, ((row - want).abs() / room.clamp(min=1e-300)).max())
     ops.check_status(dev)
