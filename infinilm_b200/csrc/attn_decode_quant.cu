@@ -34,7 +34,8 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128 || HEAD_DIM == 256, "the 8-bit d
 
 constexpr int DQ_HD = HEAD_DIM;
 constexpr int DQ_REC = kvq_record(HEAD_DIM);
-constexpr int DQ_STAGES = HEAD_DIM > 128 ? 2 : 3;   // records of a warp's ring: more gain nothing (108, 110 us with three and four)
+constexpr int DQ_STAGES = 2;                      // records of a warp's ring: three gain nothing (105, 112 us for 64 requests of up to 8,192 tokens, 32 heads on 8 of 128)
+constexpr int DQ_CH = HEAD_DIM / 16;               // pieces of 16 columns of a head
 constexpr int DQ_KG = HEAD_DIM / 64;              // groups of four product steps of Q.K^T
 constexpr int DQ_MT = HEAD_DIM / 16;              // tiles of 16 columns of V
 constexpr int DQ_VB = HEAD_DIM / 8 < 16 ? HEAD_DIM / 8 : 16;      // columns a lane takes of a key row at a time
@@ -43,14 +44,15 @@ constexpr int DQ_WARPS = 4;
 // Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 13.7 / 11.0 (fewer parts to add up); one of 512 8.0 / 8.6, of 8,192 9.9 / 10.0.
 constexpr int DQ_LEAST = 8;
 constexpr int DQ_OS = HEAD_DIM + 4;
-// Shared memory of a block: the warps' rings, over them the merge; the rings' barriers behind.
+// Shared memory of a block: the warps' rings, over them the merge; behind, the rings' barriers and the stretch's queries.
 __host__ __device__ constexpr int dq_bars(int rows) {
     const int merge = DQ_WARPS * rows * (DQ_OS + 2) * 4 + rows * 8, pipe = DQ_WARPS * DQ_STAGES * DQ_REC;
     return ((pipe > merge ? pipe : merge) + 15) / 16 * 16;
 }
-__host__ __device__ constexpr int dq_smem(int rows) { return dq_bars(rows) + DQ_WARPS * DQ_STAGES * 8; }
+__host__ __device__ constexpr int dq_q(int rows) { return dq_bars(rows) + (DQ_WARPS * DQ_STAGES * 8 + 15) / 16 * 16; }          // q's halves and the heads' factors
+__host__ __device__ constexpr int dq_smem(int rows) { return dq_q(rows) + rows * DQ_HD * 2 + rows * 4; }
 // Blocks an SM that the registers are to allow.
-constexpr int dq_per_sm(int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 1 ? 4 : 3) : (nt == 1 ? 3 : 2); }
+constexpr int dq_per_sm(int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? 4 : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
 constexpr float DQ_RAISE = 8.f;                   // the running maximum follows only when a page's is more than this above it (log2 units)
 
@@ -185,6 +187,8 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
 
     const uint32_t pipe = (uint32_t)__cvta_generic_to_shared(smem) + warp * DQ_STAGES * DQ_REC;
     const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + BARS + warp * DQ_STAGES * 8;
+    uint2* q_sm = reinterpret_cast<uint2*>(smem + dq_q(ROWS));             // [product step][lane][NT]
+    float* q_scale = reinterpret_cast<float*>(smem + dq_q(ROWS) + ROWS * DQ_HD * 2);
     const size_t page_bytes = (size_t)nkv * DQ_REC;
     if (lane == 0) {
         for (int s = 0; s < DQ_STAGES; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n" ::"r"(bars + s * 8));
@@ -209,23 +213,6 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
         const int* bt = block_table + (size_t)e * bt_stride;
         const unsigned char* recs = cache + (size_t)head * DQ_REC;
         const int n_my = dead ? 0 : max(0, (p1 - p0 - warp + DQ_WARPS - 1) / DQ_WARPS);
-        // q's rows are on their way while the pages' are asked for: head 8 j + lg, of each group of 64 columns the 16 from 16 lq on
-        uint32_t qx[NT][8 * DQ_KG];
-        const auto load_q = [&]() {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int r = 8 * j + lg;
-                const __nv_bfloat16* row = q + (size_t)e * q_stride + (size_t)(head0 + r) * DQ_HD;
-#pragma unroll
-                for (int kg = 0; kg < DQ_KG; ++kg)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint4 w = r < rows_valid ? *reinterpret_cast<const uint4*>(row + 64 * kg + 16 * lq + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-                        qx[j][8 * kg + 4 * c] = w.x, qx[j][8 * kg + 4 * c + 1] = w.y, qx[j][8 * kg + 4 * c + 2] = w.z, qx[j][8 * kg + 4 * c + 3] = w.w;
-                    }
-            }
-        };
-        if (waited) load_q();
         // Page ids of this warp's iterations, 32 at a time: lane l holds the id of iteration base + l.
         int ids_base = 0, my_ids = lane < n_my ? bt[p0 + warp + lane * DQ_WARPS] : 0;
         unsigned bad = 0;                         // bit (iteration % 32): the page is not there, its keys are masked
@@ -251,32 +238,41 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
             for (; issued < DQ_STAGES && p0 + warp + issued * DQ_WARPS < last_page; ++issued) issue(issued);
             il_pdl_wait();
             waited = true;
-            load_q();
         }
         for (; issued < DQ_STAGES; ++issued) issue(issued);
 
-        // Q as the products' right operand
-        uint32_t qf[4 * DQ_KG][NT][2];
-        il_f2 s_scale[NT];                        // what the scores of heads 8 j + 2 lq, + 1 are multiplied by (q's power of two taken back)
+        // Q as the products' right operand, in shared memory in the order in which a product step's lanes read it: head 8 j + lg, of each group of 64 columns the 16 from 16 lq on. A thread
+        // makes 16 columns of a head, the lanes of a head agree on its power of two.
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            uint32_t most = 0u;
-            const uint32_t* x = qx[j];
+        for (int i0 = 0; i0 < ROWS * DQ_CH; i0 += DQ_WARPS * 32) {
+            const int item = i0 + threadIdx.x, r = item / DQ_CH, c = item % DQ_CH;
+            if (ROWS * DQ_CH < DQ_WARPS * 32 && item >= ROWS * DQ_CH) break;       // (whole warps)
+            uint32_t x[8], most = 0u;
+            {
+                const uint4* at = reinterpret_cast<const uint4*>(q + (size_t)e * q_stride + (size_t)(head0 + r) * DQ_HD + 16 * c);
+                const uint4 u = r < rows_valid ? at[0] : make_uint4(0u, 0u, 0u, 0u), w = r < rows_valid ? at[1] : make_uint4(0u, 0u, 0u, 0u);
+                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+            }
 #pragma unroll
-            for (int c = 0; c < 8 * DQ_KG; ++c) most = max(most, max(x[c] & 0x7fffu, x[c] >> 16 & 0x7fffu));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            for (int k = 0; k < 8; ++k) most = max(most, max(x[k] & 0x7fffu, x[k] >> 16 & 0x7fffu));
+#pragma unroll
+            for (int k = 1; k < DQ_CH; k <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, k));
             const int ex = max((int)(most >> 7) - 127, -100);
-            const float up = __int_as_float((127 + 14 - ex) << 23), back = scale_log2 * __int_as_float((127 - 14 + ex) << 23);
-            s_scale[j] = il_f2_make(__shfl_sync(0xffffffffu, back, 8 * lq), __shfl_sync(0xffffffffu, back, 8 * lq + 4));
+            const float up = __int_as_float((127 + 14 - ex) << 23);
+            if (c == 0) q_scale[r] = scale_log2 * __int_as_float((127 - 14 + ex) << 23);
 #pragma unroll
-            for (int i = 0; i < 4 * DQ_KG; ++i) {
-                const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i]), b = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * i + 1]);
+            for (int k = 0; k < 4; ++k) {
+                const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * k]), b = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * k + 1]);
                 const float x0 = __low2float(a) * up, x1 = __high2float(a) * up, x2 = __low2float(b) * up, x3 = __high2float(b) * up;
-                qf[i][j][0] = KIND == KVQ_E4M3 ? dq_pack_half(x0, x1) : dq_pack_half(x0, x2);          // (in the order in which K's codes come)
-                qf[i][j][1] = KIND == KVQ_E4M3 ? dq_pack_half(x2, x3) : dq_pack_half(x1, x3);
+                // (in the order in which K's codes come)
+                q_sm[((4 * (c / 4) + k) * 32 + (r % 8) * 4 + c % 4) * NT + r / 8] =
+                    KIND == KVQ_E4M3 ? make_uint2(dq_pack_half(x0, x1), dq_pack_half(x2, x3)) : make_uint2(dq_pack_half(x0, x2), dq_pack_half(x1, x3));
             }
         }
+        __syncthreads();
+        il_f2 s_scale[NT];                        // what the scores of heads 8 j + 2 lq, + 1 are multiplied by (q's power of two taken back)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s_scale[j] = il_f2_make(q_scale[8 * j + 2 * lq], q_scale[8 * j + 2 * lq + 1]);
 
         float o[DQ_MT][NT][4];                    // columns 2 t, 2 t + 1 of lane lg's (elements 0, 1 and 2, 3), heads 8 j + 2 lq, + 1
 #pragma unroll
@@ -317,8 +313,15 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                     uint32_t a[4];
                     dq_halves<KIND>(c[0][i], a[0], a[2]);
                     dq_halves<KIND>(c[1][i], a[1], a[3]);
+                    uint2 qf[NT];
+                    if constexpr (NT == 2) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(q_sm + ((4 * kg + i) * 32 + lane) * 2);
+                        qf[0] = make_uint2(w.x, w.y), qf[1] = make_uint2(w.z, w.w);
+                    } else {
+                        qf[0] = q_sm[(4 * kg + i) * 32 + lane];
+                    }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) dq_mma(i & 1 ? s1[j] : s[j], a, qf[4 * kg + i][j][0], qf[4 * kg + i][j][1]);
+                    for (int j = 0; j < NT; ++j) dq_mma(i & 1 ? s1[j] : s[j], a, qf[j].x, qf[j].y);
                 }
             }
 #pragma unroll
@@ -642,29 +645,30 @@ struct DqArgs {
     float scale;
 };
 IL_EXPORT int il_attn_decode_quant(const DqArgs* args) {
-    const auto [q, q_stride, out, cache, block_table, entry_kvlen, o_part, ml_part, status, stream, kind, bt_stride, n_decode, nh, nkv, hd, window, n_blocks, early, scale] = *args;
+    const DqArgs& a = *args;
+    const int kind = a.kind, n_decode = a.n_decode, nh = a.nh, nkv = a.nkv, hd = a.hd, n_blocks = a.n_blocks;
     if (n_decode <= 0) return IL_OK;
     if (hd != HEAD_DIM) return IL_UNSUPPORTED;
-    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !status) return IL_BAD_ARG;
+    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !a.status) return IL_BAD_ARG;
     const int group = nh / nkv, rows = group <= 8 ? 8 : 16, row_tiles = (group + rows - 1) / rows, units = nkv * row_tiles;
-    if ((long long)n_decode * units * bt_stride > 0x7fffffffLL || n_blocks > 0x3fffffff) return IL_UNSUPPORTED;   // (pages of all units are counted in 32 bits)
-    if (n_blocks > 0 && (!o_part || !ml_part)) return IL_BAD_ARG;
-    if ((((uintptr_t)cache | (uintptr_t)q | (uintptr_t)out) & 15) || (q_stride & 7) || q_stride < (long long)nh * hd) return IL_BAD_ARG;
+    if ((long long)n_decode * units * a.bt_stride > 0x7fffffffLL || n_blocks > 0x3fffffff) return IL_UNSUPPORTED;   // (pages of all units are counted in 32 bits)
+    if (n_blocks > 0 && (!a.o_part || !a.ml_part)) return IL_BAD_ARG;
+    if ((((uintptr_t)a.cache | (uintptr_t)a.q | (uintptr_t)a.out) & 15) || (a.q_stride & 7) || a.q_stride < (long long)nh * hd) return IL_BAD_ARG;
     int dev = 0;
     cudaGetDevice(&dev);
     const int rc = dq_prepare(dev);
     if (rc != IL_OK) return rc;
     const int whole = n_blocks == 0;
     cudaError_t e = dq_pick(kind, group, [&](auto kernel, int smem) {
-        return il_launch(kernel, dim3(whole ? n_decode * units : n_blocks), dim3(DQ_WARPS * 32), (size_t)smem, stream, (const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache, block_table, bt_stride,
-                         entry_kvlen, n_decode, nh, nkv, group, row_tiles, scale * 1.4426950408889634f, window, whole, o_part, ml_part, (__nv_bfloat16*)out, status, early);
+        return il_launch(kernel, dim3(whole ? n_decode * units : n_blocks), dim3(DQ_WARPS * 32), (size_t)smem, a.stream, (const __nv_bfloat16*)a.q, a.q_stride, (const unsigned char*)a.cache, a.block_table, a.bt_stride,
+                         a.entry_kvlen, n_decode, nh, nkv, group, row_tiles, a.scale * 1.4426950408889634f, a.window, whole, a.o_part, a.ml_part, (__nv_bfloat16*)a.out, a.status, a.early);
     });
     if (e == cudaSuccess && !whole) {
         // warps a row by the parts that a unit has if the requests are alike
         const int parts = n_blocks / (n_decode * units), n_rows = n_decode * nh;
         const auto merge = [&](auto kernel, int blocks, int threads) {
-            return il_launch(kernel, dim3(blocks), dim3(threads), (size_t)0, stream, (const float*)o_part, (const float*)ml_part, entry_kvlen, n_decode, nh, group, rows, row_tiles, units, window, n_blocks,
-                             (__nv_bfloat16*)out);
+            return il_launch(kernel, dim3(blocks), dim3(threads), (size_t)0, a.stream, (const float*)a.o_part, (const float*)a.ml_part, a.entry_kvlen, n_decode, nh, group, rows, row_tiles, units, a.window, n_blocks,
+                             (__nv_bfloat16*)a.out);
         };
         e = parts > 64 ? merge(attn_decode_quant_merge_kernel<16>, n_rows, 512) : parts > 8 ? merge(attn_decode_quant_merge_kernel<4>, n_rows, 128)
                                                                                 : merge(attn_decode_quant_merge_kernel<1>, (n_rows + 3) / 4, 128);
