@@ -267,23 +267,48 @@ IL_EXPORT int il_rope_store_quant(const KvqStoreArgs* args) {
     return IL_OK;
 }
 
-// A block a page of a request. Pages in front of the one that holds the lowest position the request's portion sees (its first new token's, by the mask) and behind the last
+// The pages of a request that its portion sees: the first of them, and how many.
+__device__ __forceinline__ int kvu_seen(const int* entry_kvlen, const int* entry_qstart, int window, int e, int width, int* first) {
+    const int kvlen = entry_kvlen[e];
+    *first = entry_qstart ? il_mask_lo(max(kvlen - (entry_qstart[e + 1] - entry_qstart[e]), 0), window) / KVQ_PAGE : 0;
+    return max(min((kvlen + KVQ_PAGE - 1) / KVQ_PAGE, width) - *first, 0);
+}
+
+// A block a page of a request. room > 0: the pages that are seen lie one behind the other, request after request, up to `room` of them, and `table` says where (0 for the others: in bounds for who looks all the same; pages for
+// which no room is left set *status); else page p of the i-th request lies at i * width + p. Pages in front of the one that holds the lowest position the request's portion sees (its first new token's, by the mask) and behind the last
 // are left as they are, slots behind the request's end become zeros. A thread makes 16 bytes of output at a time, KVU_AHEAD of them at once: bound by memory, what matters is loads under
 // way. HD 0: any head size. 16 requests of up to 8,192 tokens, 8 kv heads of 128, e4m3 to bfloat16, us: one at a time 85.4,
 // two 80.2, four 79.9.
 constexpr int KVU_AHEAD = 4;
 template <typename TO, int KIND, int HD>
 __global__ void __launch_bounds__(256) kv_unpack_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
-                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key) {
+                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room, int* status) {
     il_pdl_begin();
     constexpr int VEC = 16 / sizeof(TO);
     const int hd = HD ? HD : hd_arg;
     const int i = blockIdx.y, e = first_entry + i, p = blockIdx.x;
-    const size_t to = (size_t)i * gridDim.x + p;
-    if (table && threadIdx.x == 0) table[(size_t)e * gridDim.x + p] = (int)to;
-    const int kvlen = entry_kvlen[e];
-    const int lo = entry_qstart ? il_mask_lo(max(kvlen - (entry_qstart[e + 1] - entry_qstart[e]), 0), window) : 0;
-    if (p < lo / KVQ_PAGE || p >= (kvlen + KVQ_PAGE - 1) / KVQ_PAGE) return;
+    int first;
+    const int n_seen = kvu_seen(entry_kvlen, entry_qstart, window, e, gridDim.x, &first), kvlen = entry_kvlen[e];
+    const bool seen = p >= first && p - first < n_seen;
+    size_t to = (size_t)i * gridDim.x + p;
+    if (room > 0 && seen) {                       // behind the pages of the requests in front
+        __shared__ int sums[8];
+        int sum = 0, f;
+        for (int k = threadIdx.x; k < i; k += 256) sum += kvu_seen(entry_kvlen, entry_qstart, window, first_entry + k, gridDim.x, &f);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += sums[k];
+        to = (size_t)sum + (p - first);
+    }
+    const bool fits = room <= 0 || to < (size_t)room;
+    if (threadIdx.x == 0) {
+        if (table) table[(size_t)e * gridDim.x + p] = room > 0 && !(seen && fits) ? 0 : (int)to;
+        if (seen && !fits) atomicExch(status, 92);
+    }
+    if (!seen || !fits) return;
     const int page = block_table[(size_t)e * bt_stride + p], rec_bytes = kvq_record(hd), n_keys = page < 0 ? 0 : min(KVQ_PAGE, kvlen - p * KVQ_PAGE);
     const unsigned char* recs = cache + (size_t)max(page, 0) * nkv * rec_bytes;
     TO* out = pages + to * 2 * nkv * KVQ_PAGE * hd;
@@ -333,19 +358,22 @@ struct KvqUnpackArgs {
     void* pages;
     int* table;
     cudaStream_t stream;
-    int kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key;
+    int* status;
+    int kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key, room;
 };
 IL_EXPORT int il_kv_unpack(const KvqUnpackArgs* args) {
-    const auto [cache, block_table, entry_kvlen, entry_qstart, pages, table, stream, kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key] = *args;
+    const auto [cache, block_table, entry_kvlen, entry_qstart, pages, table, stream, status, kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key,
+                room] = *args;
     const int n = n_entries - first_entry;
     if (n <= 0 || width <= 0) return IL_OK;
     if (hd > 256 || n > 65535) return IL_UNSUPPORTED;
     if (nkv <= 0 || hd <= 0 || hd % 16 || width > bt_stride || first_entry < 0 || (((uintptr_t)cache | (uintptr_t)pages) & 15)) return IL_BAD_ARG;
     if ((long long)n * width > 0x7fffffffLL) return IL_UNSUPPORTED;
+    if (room < 0 || (room > 0 && (!table || !status))) return IL_BAD_ARG;
     if ((kind != KVQ_E4M3 && kind != KVQ_INT8) || (out_kind != IL_F32 && out_kind != IL_BF16)) return IL_BAD_ARG;
 #define KVU_OF(TO, KIND, HD)                                                                                                                                \
     IL_LAUNCH((kv_unpack_kernel<TO, KIND, HD>), dim3(width, n), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen, entry_qstart, \
-              window, first_entry, nkv, hd, (TO*)pages, table, told_by_key)
+              window, first_entry, nkv, hd, (TO*)pages, table, told_by_key, room, status)
 #define KVU_GO(TO, KIND)                                 \
     do {                                                 \
         if (hd == 64) KVU_OF(TO, KIND, 64);              \

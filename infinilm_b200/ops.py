@@ -1026,7 +1026,7 @@ def stream_status(device) -> torch.Tensor:
 
 # What a kernel whose bounded wait ran out leaves in its stream's status word: from, to, the kernel's file.
 STATUS_CODES = ((11, 14, "gemm_tc5"), (21, 21, "attn_decode"), (30, 39, "attn_prefill_tc5"), (51, 54, "gemm_mid"), (71, 75, "gemm_f32"),
-                (81, 83, "gemm_narrow_tc5"), (91, 91, "attn_decode_quant"), (101, 109, "attn_prefill_pair"))
+                (81, 83, "gemm_narrow_tc5"), (91, 91, "attn_decode_quant"), (92, 92, "kv_quant"), (101, 109, "attn_prefill_pair"))
 
 
 def check_status(device) -> None:
@@ -1845,7 +1845,7 @@ def kv_quant_record(head_dim: int) -> int:
 
 
 # Arguments of the entry points below as the structs that they take (a ctypes call with twenty arguments of its own costs 3 us of host time, between kernels of a few microseconds).
-_STORE_ARGS, _UNPACK_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<7Q10i")
+_STORE_ARGS, _UNPACK_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<8Q11i")
 _DECODE_ARGS, _PAIR_ARGS = struct.Struct("<Qq8Q9if"), struct.Struct("<Qq7Q8if")
 _quant_fns = {}
 
@@ -1930,12 +1930,14 @@ def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tens
 
 def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_kvlen: torch.Tensor, pages: torch.Tensor,
               table: Optional[torch.Tensor] = None, entry_qstart: Optional[torch.Tensor] = None, window: Optional[int] = None,
-              first_entry: int = 0, nan_in_keys: bool = False) -> None:
+              first_entry: int = 0, nan_in_keys: bool = False, packed: bool = False) -> None:
     """Reads requests' pages of an 8-bit cache back as values: page p of entry first_entry + i goes to pages[i * width + p], `pages` being bfloat16 or
     float32 [entries * width, 2, kv_heads, 16, head_dim], the layout of a cache without codes, and `width` the block table's. Every value is exact in both types.
     Slots behind an entry's length become zeros, whole pages behind it are left as they are; so are, with `entry_qstart` (int32 [entries + 1]: an entry's new tokens
     are its last qstart[e + 1] - qstart[e]) and `window`, the pages in front of what the first new token sees. A block-table entry below 0 reads as zeros.
     `table` (int32 of block_table's shape, or None): receives the block table of `pages` for the entries from first_entry on.
+    `packed` (with `table`): the pages that are read lie one behind the other instead, entry after entry, from pages[0] on, and `table` has 0 for the others; more of them than `pages` has
+    room for are not read, and `check_status` reports it.
     `nan_in_keys`: for an attention that reads `pages` - a row of V that is NaN comes back as zeros and its row of K as NaN, so that
     who does not see the key does not get the NaN either."""
     what = "kv_unpack"
@@ -1955,13 +1957,15 @@ def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_k
             raise KernelError(f"{what}: entry_qstart int32 [entries + 1]")
     if table is not None:
         _descriptors(what, table)
-    if room < (n_entries - first_entry) * width or (table is not None and table.shape != (n_entries, width)):
-        raise KernelError(f"{what}: room for entries * width pages, table of the block table's shape")
+    if (table is None if packed else room < (n_entries - first_entry) * width) or (table is not None and table.shape != (n_entries, width)):
+        raise KernelError(f"{what}: room for entries * width pages (or packed ones and a table), table of the block table's shape")
+    if packed and room == 0:
+        raise KernelError(f"{what}: room for a page at least")
     d = _on_one_device(what, cache, block_table, entry_kvlen, pages, *(t for t in (table, entry_qstart) if t is not None))
     f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
     _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(), 0 if entry_qstart is None else entry_qstart.data_ptr(), pages.data_ptr(),
-                               0 if table is None else table.data_ptr(), _raw_stream(d), k, width, int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
-                               kind_of(pages.dtype), int(nan_in_keys))), what)
+                               0 if table is None else table.data_ptr(), _raw_stream(d), _status_ptr(d) if packed else 0, k, width, int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
+                               kind_of(pages.dtype), int(nan_in_keys), room if packed else 0)), what)
 
 
 _resident_quant = {}
@@ -1995,7 +1999,7 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     token at position entry_kvlen[i] - 1 and sees the keys up to itself, of the last `window` positions if given (negative: of its run of -window positions).
     `out` bfloat16 [rows, heads * head_dim]; head_dim 64, 128 or 256. A row that sees no key gets zeros; a block-table entry below 0 is never followed, its keys count as masked.
     max_kvlen: no entry is longer (what the number of blocks is planned for; any bound gives right results).
-    ws: a `Workspace` for the parts of sums that several blocks make. cached_before: the caller vouches that lengths, block tables and all pages but the newest token's were written before
+    ws: a `Workspace` for the parts of sums that several blocks make, used by one stream at a time. cached_before: the caller vouches that lengths, block tables and all pages but the newest token's were written before
     the kernel in front of this call began; they are then read while that kernel still runs."""
     what = "attention_decode_quant"
     if n_decode <= 0:
@@ -2039,6 +2043,12 @@ def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     return 2 * max(1, 128 // group) if head_dim <= 128 else max(1, prefill_tc5_rows(head_dim) // group)
 
 
+def unpacked_room(cache: torch.Tensor, n_entries: int, width: int) -> int:
+    """Pages that reading back n_entries requests takes at most, packed: what their block tables can name, and no more than the cache has (a page belongs to one request; entries
+    that only pad a step have one page each)."""
+    return max(1, min(n_entries * width, cache.shape[0] + n_entries))
+
+
 def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype):
     """A workspace's pages for `kv_unpack` ([n_pages, 2, kv_heads, 16, head_dim]) and, for bfloat16, their tensor map (see `kv_tensor_map`; None where there is none)."""
     per = 2 * n_kv_heads * KV_QUANT_PAGE * head_dim
@@ -2059,12 +2069,14 @@ def _unpacked_map(ws, n_pages: int, n_kv_heads: int, head_dim: int) -> Optional[
 
 def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_qstart: torch.Tensor,
                             entry_kvlen: torch.Tensor, first_entry: int, n_entries: int, n_tiles_total: int, n_heads: int, n_kv_heads: int, head_dim: int,
-                            scale: float, window: Optional[int], ws, n_tiles_rule: Optional[int] = None) -> None:
+                            scale: float, window: Optional[int], ws, n_tiles_rule: Optional[int] = None, room: Optional[int] = None) -> None:
     """Causal attention of the new tokens of entries [first_entry, n_entries) over an 8-bit cache that holds their keys already: entry e's rows of `q` (bfloat16
     [T, >= heads * head_dim], contiguous, the queries in the first columns) are qstart[e] .. qstart[e + 1], its last tokens. `out` bfloat16 [T, heads * head_dim]; rows of
     other entries are left as they are. `window` as in `attention_decode_quant`; head_dim 64, 128 or 256, at most 128 query heads a kv head.
     n_tiles_total = sum over these entries of ceil(new tokens / prefill_quant_tokens(...)); n_tiles_rule as in `attention_prefill_tc5`. ws: a `Workspace` that holds the requests' pages
-    as bfloat16 meanwhile (entries * block-table width pages of one layer)."""
+    as bfloat16 meanwhile (`room` pages of one layer), used by one stream at a time.
+    room: the requests see no more pages together (None: entries * block-table width; requests that share no pages have `unpacked_room`); rows that see what is behind it are then wrong, and `check_status` reports it.
+    The keys of a page that is not there (a block-table entry below 0) are zeros."""
     what = "attention_prefill_quant"
     if n_entries <= first_entry or n_tiles_total <= 0:
         return
@@ -2081,7 +2093,7 @@ def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Ten
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_qstart int32 [entries + 1], entry_kvlen int32 [entries], first_entry one of them")
     d = _on_one_device(what, q, out, cache, block_table, entry_qstart, entry_kvlen)
     width, w, stream = block_table.shape[1], int(window or 0), _raw_stream(d)
-    n_pages = (n_entries - first_entry) * width
+    n_pages = (n_entries - first_entry) * width if room is None else max(1, min(int(room), (n_entries - first_entry) * width))
     kv_map = _unpacked_map(ws, n_pages, n_kv_heads, head_dim)
     if kv_map is None or not _has_third_map(kv_map):
         raise KernelError(f"{what}: the driver has no tensor map for this cache")
@@ -2089,7 +2101,7 @@ def attention_prefill_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Ten
     qstart, kvlen = entry_qstart.data_ptr(), entry_kvlen.data_ptr()
     f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
     _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), kvlen, qstart, ws.address("kv_unpacked", n_pages * 32 * n_kv_heads * head_dim, torch.bfloat16),
-                     table, stream, k, width, w, first_entry, n_entries, width, n_kv_heads, head_dim, BF16, 1)), what)
+                     table, stream, _status_ptr(d), k, width, w, first_entry, n_entries, width, n_kv_heads, head_dim, BF16, 1, n_pages)), what)
     rule = n_tiles_total if n_tiles_rule is None else n_tiles_rule
     if head_dim <= 128 and rule * n_kv_heads >= PAIR_FROM:
         f = _quant_fns.get(("il_attn_prefill_pair", head_dim)) or _quant_fn("il_attn_prefill_pair", "attn_prefill_pair", head_dim)

@@ -86,7 +86,7 @@ class PagedAttend:
 
     def run_quant(self, qkv, out, ctx, cache) -> None:
         """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and `run` attends over those."""
-        n_dec, E = ctx.n_decode, ctx.n_entries
+        n_dec, E, width = ctx.n_decode, ctx.n_entries, cache.block_table.shape[1]
         fast = (self.dtype == torch.bfloat16 and not self.force_plain and self.hd in ops.QUANT_HEAD_DIMS and self.sink is None and self.dist_bias is None
                 and not self.sigmoid and self.cap is None)
         if fast and n_dec > 0:
@@ -97,12 +97,12 @@ class PagedAttend:
         if fast and self.prefill_kernel != "mma" and ops.prefill_tc5_ok(self.hd, self.nh // self.nkv, cache.page_size):
             per = ops.prefill_quant_tokens(self.nh, self.nkv, self.hd)
             ops.attention_prefill_quant(qkv, out, cache.storage, cache.quant, cache.block_table, ctx.entry_qstart, ctx.entry_kvlen, n_dec, E, ctx.prompt_tiles(per),
-                                        self.nh, self.nkv, self.hd, self.scale, self.mask_arg, ctx.ws, n_tiles_rule=(qkv.shape[0] - n_dec + per - 1) // per + E - n_dec - 1)
+                                        self.nh, self.nkv, self.hd, self.scale, self.mask_arg, ctx.ws, n_tiles_rule=(qkv.shape[0] - n_dec + per - 1) // per + E - n_dec - 1,
+                                        room=ops.unpacked_room(cache.storage, E - n_dec, width))
             return
-        width = cache.block_table.shape[1]
-        pages, tma_map = ops.unpacked_cache(ctx.ws, E * width, self.nkv, self.hd, self.dtype)
+        pages, tma_map = ops.unpacked_cache(ctx.ws, ops.unpacked_room(cache.storage, E, width), self.nkv, self.hd, self.dtype)
         table = ctx.ws.flat("kv_unpacked_table", E * width, torch.int32).view(E, width)
-        ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, nan_in_keys=True)
+        ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, nan_in_keys=True, packed=True)
         self.run(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None))
 
     def run(self, qkv, out, ctx, cache) -> None:

@@ -227,6 +227,51 @@ def test_unpack_gives_the_values_exactly(cuda_device, kind, dtype, nkv, hd):
     check(torch.cat([torch.full_like(got[:2], 77.0), got[:5]]), [9, 9] + first[2:], lambda e, p, w: None)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [5, 300])
+def test_unpack_packed(cuda_device, kind, n):
+    """The pages that are seen one behind the other, for more requests than a block has threads too; what has no room is left out and reported."""
+    ops, dev = _ops(), cuda_device
+    nkv, hd = 1, 64
+    g = torch.Generator().manual_seed(n)
+    kvlens = [0, 40, 16, 1, 33] + torch.randint(0, 50, (n - 5,), generator=g).tolist()
+    new = [min(k, 2) for k in kvlens]
+    rows, n_pages = _tables(kvlens, 1, 21, width=5)
+    rec, val = _cache(n_pages, nkv, hd, kind, 22)
+    qs = [0]
+    for x in new:
+        qs.append(qs[-1] + x)
+    window = 10
+    first = [max(0, k - x - window + 1) // 16 for k, x in zip(kvlens, new)]
+    seen = [max(0, (k + 15) // 16 - f) for k, f in zip(kvlens, first)]
+    total = sum(seen[1:])
+    tab, kvl = _i32(rows, dev), _i32(kvlens, dev)
+    ops.check_status(dev)
+    for room in (total, total + 3, total - 1):
+        pages, table = torch.full((room + 1, 2, nkv, 16, hd), 77.0, device=dev), torch.full_like(tab, -5)
+        ops.kv_unpack(rec.to(dev), kind, tab, kvl, pages[:room], table, entry_qstart=_i32(qs, dev), window=window, first_entry=1, packed=True)
+        at = 0
+        got, where = pages.cpu().double(), table.cpu()
+        for e in range(1, n):
+            for p in range(5):
+                if not first[e] <= p < first[e] + seen[e]:
+                    assert where[e, p] == 0
+                    continue
+                if at >= room:
+                    assert where[e, p] == 0
+                else:
+                    assert where[e, p] == at
+                    k = min(16, kvlens[e] - 16 * p)
+                    assert torch.equal(got[at][:, :, :k], val[rows[e][p]].transpose(0, 1)[:, :, :k]) and not got[at][:, :, k:].any()
+                at += 1
+        assert (got[min(at, room):] == 77.0).all() and (where[0] == -5).all()
+        if room < total:
+            with pytest.raises(ops.KernelError, match="kv_quant"):
+                ops.check_status(dev)
+        else:
+            ops.check_status(dev)
+
+
 # ---- single tokens -----------------------------------------------------------------------------------------------------------
 def _decode_check(out, q, val, rows, kvlens, nh, hd, scale, window):
     for e, n in enumerate(kvlens):
@@ -403,6 +448,33 @@ def test_prompt_portions_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd,
             room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -8 + 2.0 ** -14)
             assert ((row - want).abs() <= room).all(), (e, i, ((row - want).abs() / room.clamp(min=1e-300)).max())
     ops.check_status(dev)
+
+
+@pytest.mark.parametrize("pair_from", [0, 1 << 30])
+@pytest.mark.parametrize("window", [None, 40])
+def test_prompts_that_share_pages_and_prompts_that_do_not(cuda_device, monkeypatch, pair_from, window):
+    """More pages seen than the cache has, as requests share them; and the room that requests with pages of their own need at most, which gives the same bits."""
+    ops, dev = _ops(), cuda_device
+    monkeypatch.setattr(ops, "PAIR_FROM", pair_from)
+    nh, nkv, hd, E, n, kvlen = 4, 2, 64, 9, 5, 100
+    rows, n_pages = _tables([kvlen], 0, 12)
+    rec, _ = _cache(n_pages, nkv, hd, "int8", 13, spread=0.5)
+    q = torch.randn((n, nh * hd), generator=torch.Generator().manual_seed(14)).to(torch.bfloat16).to(dev)
+    per = ops.prefill_quant_tokens(nh, nkv, hd)
+
+    def run(entries, **kw):
+        out = torch.full((entries * n, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
+        ops.attention_prefill_quant(q.repeat(entries, 1), out, rec.to(dev), "int8", _i32(rows * entries, dev), _i32([i * n for i in range(entries + 1)], dev), _i32([kvlen] * entries, dev),
+                                    0, entries, entries * ((n + per - 1) // per), nh, nkv, hd, 0.125, window, _ws(dev), **kw)
+        return out
+    one, many = run(1), run(E)
+    assert torch.equal(many.view(E, n, nh * hd), one.expand(E, n, nh * hd))
+    cache = rec.to(dev)
+    assert torch.equal(run(1, room=ops.unpacked_room(cache, 1, len(rows[0]))), one)
+    ops.check_status(dev)
+    run(2, room=(3 if window else 8))
+    with pytest.raises(ops.KernelError, match="kv_quant"):
+        ops.check_status(dev)
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -68,6 +68,8 @@ CASES = [
     (_unpack, dict(pages=torch.zeros((4, 2, NKV, 16, HD + 16))), "cache uint8"),
     (_unpack, dict(pages=torch.zeros((4, 2, NKV, HD, 16)).transpose(3, 4)), "contiguous"),
     (_unpack, dict(table=_i(2, 3)), "table"),
+    (_unpack, dict(packed=True), "a table"),
+    (_unpack, dict(packed=True, table=_i(2, 2), pages=torch.zeros((0, 2, NKV, 16, HD))), "a page at least"),
     (_unpack, dict(first_entry=3), "first_entry"),
     (_unpack, dict(first_entry=-1), "first_entry"),
     (_unpack, dict(entry_kvlen=_i(1)), "entry_kvlen"),
