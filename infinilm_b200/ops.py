@@ -1868,21 +1868,25 @@ def _quant_cache(what: str, cache: torch.Tensor, kind: str, n_kv_heads: int, hea
     k = KV_KINDS.get(kind)
     if k is None:
         raise KernelError(f"{what}: the cache's kind is one of {', '.join(KV_KINDS)}, not {kind!r}")
-    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[1:] != (n_kv_heads, 32 * head_dim + 32):
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[1] != n_kv_heads or shape[2] != 32 * head_dim + 32 or not cache.is_contiguous():
         raise KernelError(f"{what}: cache uint8 [pages, kv_heads, 32 * head_dim + 32], contiguous")
     return k
 
 
 def _on_one_device(what: str, *ts: torch.Tensor) -> int:
     """All on the current device, whose current stream the kernels are launched on; its number."""
+    d = ts[0].get_device()                        # (below 0: not on a GPU)
     for t in ts:
-        if not t.is_cuda:
-            _need_cuda(t)
+        if t.get_device() != d or d < 0:
+            break
+    else:
+        if d == _cur_device():
+            return d
+    _need_cuda(*ts)
     d = _cur_device()
-    for t in ts:
-        if t.get_device() != d:
-            raise KernelError(f"{what}: a tensor on {t.device}; the kernels run on the current device, cuda:{d}")
-    return d
+    t = next(t for t in ts if t.get_device() != d)
+    raise KernelError(f"{what}: a tensor on {t.device}; the kernels run on the current device, cuda:{d}")
 
 
 def _descriptors(what: str, *ts: torch.Tensor) -> None:
@@ -1904,19 +1908,19 @@ def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tens
     as they are. Each token's slot is its own: what two rows write to one slot is undefined. A token whose block-table entry is below 0 is not stored.
     A row of k or v that is not finite is stored as NaN."""
     what = "rope_store_quant"
-    nq = n_heads * head_dim
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != nq + 2 * n_kv_heads * head_dim:
+    nq, shape, strides, dtype = n_heads * head_dim, qkv.shape, qkv.stride(), qkv.dtype
+    if len(shape) != 2 or strides[1] != 1 or shape[1] != nq + 2 * n_kv_heads * head_dim:
         raise KernelError(f"{what}: qkv [T, (heads + 2 kv_heads) * head_dim], columns side by side")
-    T = qkv.shape[0]
-    if q_out.shape != (T, nq) or q_out.dtype is not qkv.dtype or q_out.stride(1) != 1:
+    T, row, q_strides = shape[0], strides[0], q_out.stride()
+    if q_out.shape != (T, nq) or q_out.dtype is not dtype or q_strides[1] != 1:
         raise KernelError(f"{what}: q_out [T, heads * head_dim] of qkv's dtype, columns side by side")
     if T == 0:
         return
-    row, q_row = qkv.stride(0), q_out.stride(0)
+    q_row, table_shape = q_strides[0], block_table.shape
     if q_row < nq or row < nq:
         raise KernelError(f"{what}: rows must not overlap")
     _descriptors(what, tok_pos, tok_entry, block_table)
-    if tok_pos.numel() != T or tok_entry.numel() != T or block_table.dim() != 2:
+    if tok_pos.numel() != T or tok_entry.numel() != T or len(table_shape) != 2:
         raise KernelError(f"{what}: tok_pos and tok_entry int32 [T], block_table int32 [entries, width]")
     if rot_dim and (inv_freq is None or inv_freq.dtype is not torch.float32 or inv_freq.numel() != rot_dim // 2 or not inv_freq.is_contiguous()):
         raise KernelError(f"{what}: inv_freq float32 [rot_dim / 2]")
@@ -1924,7 +1928,7 @@ def rope_store_quant(qkv: torch.Tensor, q_out: torch.Tensor, tok_pos: torch.Tens
     d = _on_one_device(what, qkv, q_out, tok_pos, tok_entry, block_table, *([cache] if cache is not None else []), *([inv_freq] if rot_dim else []))
     f = _quant_fns.get(("il_rope_store_quant", 0)) or _quant_fn("il_rope_store_quant", "kv_quant")
     _check(f(_packed(_STORE_ARGS, what, qkv.data_ptr(), row, q_out.data_ptr(), q_row, tok_pos.data_ptr(), tok_entry.data_ptr(), block_table.data_ptr(),
-                              0 if cache is None else cache.data_ptr(), inv_freq.data_ptr() if rot_dim else 0, _raw_stream(d), kind_of(qkv.dtype), block_table.shape[1], k, T,
+                              0 if cache is None else cache.data_ptr(), inv_freq.data_ptr() if rot_dim else 0, _raw_stream(d), kind_of(dtype), table_shape[1], k, T,
                               n_heads, n_kv_heads, head_dim, rot_dim, mscale)), what)
 
 
@@ -1941,27 +1945,26 @@ def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_k
     `nan_in_keys`: for an attention that reads `pages` - a row of V that is NaN comes back as zeros and its row of K as NaN, so that
     who does not see the key does not get the NaN either."""
     what = "kv_unpack"
-    if pages.dim() != 5 or not pages.is_contiguous():
-        raise KernelError(f"{what}: pages [entries * width, 2, kv_heads, 16, head_dim], contiguous")
-    room, two, n_kv_heads, slots, head_dim = pages.shape
-    if two != 2 or slots != KV_QUANT_PAGE:
+    room, two, n_kv_heads, slots, head_dim = pages.shape if pages.dim() == 5 else (0,) * 5
+    if two != 2 or slots != KV_QUANT_PAGE or not pages.is_contiguous():
         raise KernelError(f"{what}: pages [entries * width, 2, kv_heads, 16, head_dim], contiguous")
     k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
-    _descriptors(what, block_table, entry_kvlen)
-    if block_table.dim() != 2 or not 0 <= first_entry <= block_table.shape[0] or entry_kvlen.numel() < block_table.shape[0]:
+    n_entries, width = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    if not 0 <= first_entry <= n_entries or entry_kvlen.numel() < n_entries:
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries], first_entry one of them")
-    n_entries, width = block_table.shape
+    ts = [block_table, entry_kvlen]
     if entry_qstart is not None:
-        _descriptors(what, entry_qstart)
+        ts.append(entry_qstart)
         if entry_qstart.numel() < n_entries + 1:
             raise KernelError(f"{what}: entry_qstart int32 [entries + 1]")
     if table is not None:
-        _descriptors(what, table)
+        ts.append(table)
+    _descriptors(what, *ts)
     if (table is None if packed else room < (n_entries - first_entry) * width) or (table is not None and table.shape != (n_entries, width)):
         raise KernelError(f"{what}: room for entries * width pages (or packed ones and a table), table of the block table's shape")
     if packed and room == 0:
         raise KernelError(f"{what}: room for a page at least")
-    d = _on_one_device(what, cache, block_table, entry_kvlen, pages, *(t for t in (table, entry_qstart) if t is not None))
+    d = _on_one_device(what, cache, pages, *ts)
     f = _quant_fns.get(("il_kv_unpack", 0)) or _quant_fn("il_kv_unpack", "kv_quant")
     _check(f(_packed(_UNPACK_ARGS, what, cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(), 0 if entry_qstart is None else entry_qstart.data_ptr(), pages.data_ptr(),
                                0 if table is None else table.data_ptr(), _raw_stream(d), _status_ptr(d) if packed else 0, k, width, int(window or 0), first_entry, n_entries, width, n_kv_heads, head_dim,
@@ -1975,10 +1978,10 @@ _resident_quant = {}
 QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES = 8, 12
 
 
-def _quant_blocks(head_dim: int, group: int, units: int, pages: int) -> int:
+def _quant_blocks(head_dim: int, group: int, units: int, pages: int, device: Optional[int] = None) -> int:
     """Blocks that the pages of `units` units (a kv head of a request with up to 8 or 16 of its `group` query heads) of at most `pages` pages are dealt out to: one wave of
     them, eight pages each at least; 0: a block a unit."""
-    key = (_cur_device(), head_dim, group > 8)
+    key = (_cur_device() if device is None else device, head_dim, group > 8)
     most = _resident_quant.get(key)
     if most is None:
         fn = build.load("attn_decode_quant", {"HEAD_DIM": head_dim}).il_attn_decode_quant_resident_blocks
@@ -2004,28 +2007,28 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     what = "attention_decode_quant"
     if n_decode <= 0:
         return
-    nq = n_heads * head_dim
-    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1 or not out.is_contiguous():
+    nq, shape, strides, out_shape, table_shape = n_heads * head_dim, q.shape, q.stride(), out.shape, block_table.shape
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or len(shape) != 2 or strides[1] != 1 or not out.is_contiguous():
         raise KernelError(f"{what}: bfloat16 q [rows, heads * head_dim] and contiguous out")
     if head_dim not in QUANT_HEAD_DIMS or n_kv_heads <= 0 or n_heads % n_kv_heads:
         raise KernelError(f"{what}: head sizes {QUANT_HEAD_DIMS}, heads a multiple of kv_heads")
-    if out.dim() != 2 or out.shape[1] != nq or out.shape[0] < n_decode or q.shape[0] < n_decode or q.shape[1] < nq:
+    if len(out_shape) != 2 or out_shape[1] != nq or out_shape[0] < n_decode or shape[0] < n_decode or shape[1] < nq:
         raise KernelError(f"{what}: q [>= n_decode rows, >= heads * head_dim], out [>= n_decode rows, heads * head_dim]")
     k = _quant_cache(what, cache, kind, n_kv_heads, head_dim)
     _descriptors(what, block_table, entry_kvlen)
-    if block_table.dim() != 2 or block_table.shape[0] < n_decode or entry_kvlen.numel() < n_decode:
+    if len(table_shape) != 2 or table_shape[0] < n_decode or entry_kvlen.numel() < n_decode:
         raise KernelError(f"{what}: block_table int32 [entries, width], entry_kvlen int32 [entries]")
     d = _on_one_device(what, q, out, cache, block_table, entry_kvlen)
     w, seen = int(window or 0), int(max_kvlen)
     if w:
         seen = min(seen, abs(w) + KV_QUANT_PAGE)  # (a window may begin inside a page)
     group = n_heads // n_kv_heads
-    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE))
+    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE), d)
     parts = n_blocks > 0
     f = _quant_fns.get(("il_attn_decode_quant", head_dim)) or _quant_fn("il_attn_decode_quant", "attn_decode_quant", head_dim)
-    _check(f(_packed(_DECODE_ARGS, what, q.data_ptr(), q.stride(0), out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(),
+    _check(f(_packed(_DECODE_ARGS, what, q.data_ptr(), strides[0], out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(),
                                ws.address("quant_o_part", n_blocks * 32 * head_dim, torch.float32) if parts else 0,
-                               ws.address("quant_ml_part", n_blocks * 64, torch.float32) if parts else 0, _status_ptr(d), _raw_stream(d), k, block_table.shape[1], n_decode, n_heads,
+                               ws.address("quant_ml_part", n_blocks * 64, torch.float32) if parts else 0, _status_ptr(d), _raw_stream(d), k, table_shape[1], n_decode, n_heads,
                                n_kv_heads, head_dim, w, n_blocks, int(cached_before), scale)), what)
     if parts:
         count_launches(1)                         # the second kernel
