@@ -596,3 +596,122 @@ def test_another_stream(cuda_device):
         there = go()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(here, there))
+
+
+# ---- calls that are odd but allowed ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("pair_from", [0, 1 << 30])
+@pytest.mark.parametrize("window", [None, 20])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompts_beside_requests_without_tokens(cuda_device, monkeypatch, pair_from, window, hd):
+    """Entries that bring nothing, with keys or without, change no bit of the others'; a replayed call takes the lengths that it finds."""
+    ops, dev = _ops(), cuda_device
+    monkeypatch.setattr(ops, "PAIR_FROM", pair_from)
+    nh, nkv = 6, 2
+    per = ops.prefill_quant_tokens(nh, nkv, hd)
+
+    def descriptors(cached, new, width):
+        kvlens = [a + b for a, b in zip(cached, new)]
+        qs = [0]
+        for n in new:
+            qs.append(qs[-1] + n)
+        return kvlens, qs
+    cached, new = [0, 33, 0, 100, 16, 0], [0, 0, 70, 41, 1, 0]
+    kvlens, qs = descriptors(cached, new, 10)
+    rows, n_pages = _tables(kvlens, 1, 3, width=10)
+    rec, _ = _cache(n_pages, nkv, hd, "fp8_e4m3", 4, spread=0.5)
+    cache = rec.to(dev)
+    q = torch.randn((sum(new), nh * hd), generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).to(dev)
+
+    def run(out, rows, qs, kvlens, tiles, rule, ws):
+        ops.attention_prefill_quant(q, out, cache, "fp8_e4m3", rows, qs, kvlens, 0, kvlens.numel(), tiles, nh, nkv, hd, 0.1, window, ws, n_tiles_rule=rule)
+    tiles = sum((n + per - 1) // per for n in new)
+    full = torch.full_like(q, 3.0)
+    run(full, _i32(rows, dev), _i32(qs, dev), _i32(kvlens, dev), tiles, tiles, _ws(dev))
+    some = torch.full_like(q, 3.0)
+    keep = [2, 3, 4]
+    _, qs2 = descriptors([cached[e] for e in keep], [new[e] for e in keep], 10)
+    run(some, _i32([rows[e] for e in keep], dev), _i32(qs2, dev), _i32([kvlens[e] for e in keep], dev), tiles, tiles, _ws(dev))
+    assert torch.equal(full, some) and not (full == 3.0).all(1).any()
+
+    # captured for these lengths, replayed for others whose tiles are no more
+    ws, d_rows, d_qs, d_kv, out = _ws(dev), _i32(rows, dev), _i32(qs, dev), _i32(kvlens, dev), torch.full_like(q, 3.0)
+    run(out, d_rows, d_qs, d_kv, tiles, tiles, ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(out, d_rows, d_qs, d_kv, tiles, tiles, ws)
+    for other in ([0, 0, 70, 41, 1, 0], [0, 0, 5, 1, 0, 0], [0, 0, 0, 0, 0, 0], [0, 0, 30, 41, 1, 0]):
+        kvl, qs3 = descriptors(cached, other, 10)
+        d_qs.copy_(_i32(qs3, dev)), d_kv.copy_(_i32(kvl, dev)), out.fill_(3.0)
+        graph.replay()
+        want = torch.full_like(q, 3.0)
+        run(want, _i32(rows, dev), _i32(qs3, dev), _i32(kvl, dev), tiles, tiles, _ws(dev))
+        assert torch.equal(out, want) and (out[sum(other):] == 3.0).all() and not (out[:sum(other)] == 3.0).all(1).any()
+    ops.check_status(dev)
+
+
+def test_two_captured_steps_that_share_a_workspace(cuda_device):
+    """A long and a short step of single tokens, captured over one workspace and replayed in turn: each gives what it gives alone."""
+    ops, dev = _ops(), cuda_device
+    nh, nkv, hd = 16, 2, 64
+    ws, steps = _ws(dev), []
+    for i, kvlens in enumerate(([3000, 17, 1200], [300] * 5)):
+        rows, n_pages = _tables(kvlens, 0, i)
+        rec, _ = _cache(n_pages, nkv, hd, "int8", i + 2)
+        q = torch.randn((len(kvlens), nh * hd), generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).to(dev)
+        steps.append((q, torch.zeros_like(q), rec.to(dev), "int8", _i32(rows, dev), _i32(kvlens, dev), len(kvlens), nh, nkv, hd, 0.1, None, max(kvlens)))
+    alone = []
+    for a in steps:
+        ops.attention_decode_quant(*a, ws)
+        alone.append(a[1].clone())
+    torch.cuda.synchronize()
+    graphs = []
+    for a in steps:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.attention_decode_quant(*a, ws)
+    for i in (0, 1, 0, 0, 1):
+        steps[i][1].zero_()
+        graphs[i].replay()
+        assert torch.equal(steps[i][1], alone[i])
+    ops.check_status(dev)
+
+
+@pytest.mark.parametrize("blocks", [None, 0])
+@pytest.mark.parametrize("nh", [4, 12])
+def test_decode_of_a_thousand_requests(cuda_device, monkeypatch, blocks, nh):
+    """More requests than a warp's lanes count at a time, many without a key, next to long ones."""
+    ops, dev = _ops(), cuda_device
+    nkv, hd, n = 1, 64, 1000
+    if blocks is not None:
+        monkeypatch.setattr(ops, "_quant_blocks", lambda *a: blocks)
+    g = torch.Generator().manual_seed(9)
+    kvlens = [0 if i % 3 == 0 else int(torch.randint(1, 90, (1,), generator=g)) for i in range(n)]
+    kvlens[500], kvlens[999] = 2500, 700
+    rows, n_pages = _tables(kvlens, 0, 7)
+    rec, val = _cache(n_pages, nkv, hd, "fp8_e4m3", 8)
+    q = torch.randn((n, nh * hd), generator=g).to(torch.bfloat16)
+    out = torch.full((n, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
+    ops.attention_decode_quant(q.to(dev), out, rec.to(dev), "fp8_e4m3", _i32(rows, dev), _i32(kvlens, dev), n, nh, nkv, hd, 0.125, None, max(kvlens), _ws(dev))
+    pick = sorted({0, 1, 2, 31, 32, 33, 499, 500, 501, 998, 999, *range(7, n, 61)})
+    _decode_check(out.cpu()[pick], q[pick], val, [rows[e] for e in pick], [kvlens[e] for e in pick], nh, hd, 0.125, 0)
+    assert not out.cpu()[::3][[i for i in range(334) if kvlens[3 * i] == 0]].any()
+    ops.check_status(dev)
+
+
+def test_store_of_many_tokens_is_the_store_of_few(cuda_device):
+    """Warps a token are chosen by the number of tokens: the same codes and queries either way."""
+    ops, dev = _ops(), cuda_device
+    nh, nkv, hd, T = 8, 2, 128, 6000
+    rows, n_pages = _tables([T], 0, 1)
+    qkv = torch.randn((T, (nh + 2 * nkv) * hd), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    pos, entry, tab = torch.arange(T, dtype=torch.int32, device=dev), torch.zeros(T, dtype=torch.int32, device=dev), _i32(rows, dev)
+    freq = (10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)).float().to(dev)
+    got = []
+    for step in (T, 37):
+        cache, q = torch.zeros((n_pages, nkv, 32 * hd + 32), dtype=torch.uint8, device=dev), torch.zeros((T, nh * hd), dtype=torch.bfloat16, device=dev)
+        for a in range(0, T, step):
+            b = min(T, a + step)
+            ops.rope_store_quant(qkv[a:b], q[a:b], pos[a:b], entry[a:b], tab, cache, "int8", nh, nkv, hd, hd, freq, 1.0)
+        got.append((cache, q))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
