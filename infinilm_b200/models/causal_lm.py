@@ -7,6 +7,7 @@ is ours: the head runs only on the rows whose logits are wanted.
 """
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -24,7 +25,7 @@ def quantise_caches(spec: ModelSpec, kind: Optional[str]) -> None:
     for i, ls in enumerate(spec.layers):
         if not part_class("mixer", ls.mixer.kind).takes_quant_cache:
             raise ConfigError(f"kv_cache_dtype {kind}: the cache of layer {i}'s mixer ({ls.mixer.kind}) has no 8-bit form")
-        ls.mixer.params["kv_cache"] = kind
+        spec.layers[i] = replace(ls, mixer=replace(ls.mixer, params={**ls.mixer.params, "kv_cache": kind}))     # (a description may hand out one part for several models)
 
 
 class CausalLM:

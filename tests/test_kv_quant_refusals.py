@@ -152,6 +152,19 @@ def test_a_model_whose_layers_have_no_such_cache_is_refused():
         CausalLM(spec, torch.bfloat16)
 
 
+def test_descriptions_that_share_a_part():
+    """Another model made of the same part keeps its own kind of cache."""
+    from dataclasses import replace
+
+    from infinilm_b200.config.registry import config_from_json, describe_model
+    from infinilm_b200.models.causal_lm import quantise_caches
+    from tiny_configs import tiny_b
+    one = describe_model(config_from_json(tiny_b()))
+    two = replace(one, layers=list(one.layers))
+    quantise_caches(one, "int8")
+    assert one.layers[0].mixer.params["kv_cache"] == "int8" and two.layers[0].mixer.params.get("kv_cache") is None
+
+
 def test_pages_of_such_a_cache():
     from infinilm_b200.cache.manager import CacheManager
     from infinilm_b200.parts.spec import CacheNeed
