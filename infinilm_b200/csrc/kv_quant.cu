@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv,
         }
     };
     load(part * HEADS);                           // on their way while the angles are made
-    float c[8], s[8];
+    il_f2 c[4], s[4];
     if (rot) {
         float co[OWN], so[OWN];
 #pragma unroll
@@ -97,7 +97,11 @@ __global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv,
             if (j < pairs) kvq_angle(pos, inv_freq[at], mscale, &co[i], &so[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = __shfl_sync(0xffffffffu, co[i % OWN], i / OWN * PER + j), s[i] = __shfl_sync(0xffffffffu, so[i % OWN], i / OWN * PER + j);
+        for (int i = 0; i < 8; i += 2) {
+            const int a = i / OWN * PER + j, b = (i + 1) / OWN * PER + j;
+            c[i / 2] = il_f2_make(__shfl_sync(0xffffffffu, co[i % OWN], a), __shfl_sync(0xffffffffu, co[(i + 1) % OWN], b));
+            s[i / 2] = il_f2_make(__shfl_sync(0xffffffffu, so[i % OWN], a), __shfl_sync(0xffffffffu, so[(i + 1) % OWN], b));
+        }
     }
     for (int first = part * HEADS; first < rows; first += KVS_AHEAD * wpt * HEADS) {
         KvqEight<TA> wa[KVS_AHEAD], wb[KVS_AHEAD];
@@ -115,11 +119,13 @@ __global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv,
             const TA *pa = reinterpret_cast<const TA*>(&wa[u]), *pb = reinterpret_cast<const TA*>(&wb[u]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = il_to_f(pa[i]), y[i] = il_to_f(pb[i]);
-            if (turns) {
+            if (turns) {                          // (kvq_lo and kvq_hi, two at a time)
+                const il_f2 minus = il_f2_dup(-1.f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x1 = x[i], x2 = y[i];
-                    x[i] = kvq_lo(x1, x2, c[i], s[i]), y[i] = kvq_hi(x1, x2, c[i], s[i]);
+                for (int i = 0; i < 8; i += 2) {
+                    const il_f2 x1 = il_f2_make(x[i], x[i + 1]), x2 = il_f2_make(y[i], y[i + 1]);
+                    il_f2_get(il_f2_fma(il_f2_mul(x2, s[i / 2]), minus, il_f2_mul(x1, c[i / 2])), x[i], x[i + 1]);
+                    il_f2_get(il_f2_add(il_f2_mul(x2, c[i / 2]), il_f2_mul(x1, s[i / 2])), y[i], y[i + 1]);
                 }
             }
             if (mine && r < nh) {
