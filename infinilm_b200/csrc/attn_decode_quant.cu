@@ -19,7 +19,9 @@
 //   Work: the pages that request e sees, once for each of its units (a kv head, and of its query heads up to 8 NT), one behind the other over requests and units. Block b
 //   takes pages b S .. (b + 1) S of that row, S = all / blocks: requests of any lengths fill the blocks alike. A stretch of one unit is computed by the block's four warps
 //   (warp w takes pages w, w + 4, ... of it; a page's record of a kv head is one untiled bulk copy into the warp's own ring) and merged
-//   in shared memory. A unit that lies in one block is final there, else its parts go to scratch. Short requests (`whole`): a block a unit, all of them final.
+//   in shared memory. A unit that lies in one block is final there, else its parts go to scratch. Short requests: a block a unit, all of them final
+//   (per_unit 1). In between, where one wave of blocks holds two to eight blocks a unit that are not much longer than dealt out: a cluster of them (per_unit), whose blocks read each other's parts
+//   from shared memory: no scratch, no second kernel (eight requests of 1,024 tokens, 32 heads on 8 of 128, 10.2 -> 8.1 us).
 //   (Parts added up by the block that finishes last, with fences and counts, took 8 us more than blocks that are final; the second kernel takes 2 to 3.)
 //
 // Token t (= entry t) sits at position kvlen - 1 and sees positions max(0, kvlen - window) .. kvlen - 1 (window < 0: runs of -window; 0: all). No
@@ -34,16 +36,17 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128 || HEAD_DIM == 256, "the 8-bit d
 
 constexpr int DQ_HD = HEAD_DIM;
 constexpr int DQ_REC = kvq_record(HEAD_DIM);
-constexpr int DQ_STAGES = 2;                      // records of a warp's ring: three gain nothing (105, 112 us for 64 requests of up to 8,192 tokens, 32 heads on 8 of 128)
+constexpr int DQ_STAGES = 2;                      // records of a warp's ring: three gain nothing (105, 111 us for 64 requests of up to 8,192 tokens, 32 heads on 8 of 128)
 constexpr int DQ_CH = HEAD_DIM / 16;               // pieces of 16 columns of a head
 constexpr int DQ_KG = HEAD_DIM / 64;              // groups of four product steps of Q.K^T
 constexpr int DQ_MT = HEAD_DIM / 16;              // tiles of 16 columns of V
 constexpr int DQ_VB = HEAD_DIM / 8 < 16 ? HEAD_DIM / 8 : 16;      // columns a lane takes of a key row at a time
 constexpr int DQ_NVB = HEAD_DIM / 8 / DQ_VB;      // ... and how often
 constexpr int DQ_WARPS = 4;
-// Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 13.7 / 11.0 (fewer parts to add up); one of 512 8.0 / 8.6, of 8,192 9.9 / 10.0.
+// Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 11.0 / 9.7 (fewer parts to add up); one of 512 7.4 / 7.9, of 8,192 9.4 / 8.2.
 constexpr int DQ_LEAST = 8;
 constexpr int DQ_OS = HEAD_DIM + 4;
+constexpr int DQ_CLUSTER = 8;                    // blocks of a cluster at most
 // Shared memory of a block: the warps' rings, over them the merge; behind, the rings' barriers and the stretch's queries.
 __host__ __device__ constexpr int dq_bars(int rows) {
     const int merge = DQ_WARPS * rows * (DQ_OS + 2) * 4 + rows * 8, pipe = DQ_WARPS * DQ_STAGES * DQ_REC;
@@ -145,6 +148,18 @@ __device__ __forceinline__ DqDeal dq_deal(const int* entry_kvlen, int n_decode, 
     }
     return d;
 }
+// Of block `rank` of the cluster.
+__device__ __forceinline__ float2 dq_peer2(uint32_t addr, int rank) {
+    float2 v;
+    asm volatile("{\n.reg .b32 at;\nmapa.shared::cluster.u32 at, %2, %3;\nld.shared::cluster.v2.f32 {%0,%1}, [at];\n}\n" : "=f"(v.x), "=f"(v.y) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 dq_peer4(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("{\n.reg .b32 at;\nmapa.shared::cluster.u32 at, %4, %5;\nld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [at];\n}\n"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
 // Where a unit's parts lie: its first block's second place, the others' first (a block holds at most the end of one unit and the start of another).
 __device__ __forceinline__ int dq_place(int b0, int i) { return i == 0 ? 2 * b0 + 1 : 2 * (b0 + i); }
 
@@ -163,7 +178,7 @@ __device__ __forceinline__ void dq_write(const float4& acc, float M, float L, __
 template <int KIND, int NT>
 __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quant_kernel(
     const __nv_bfloat16* q, long long q_stride, const unsigned char* cache, const int* __restrict__ block_table, int bt_stride,
-    const int* __restrict__ entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int whole, float* o_part, float* ml_part,
+    const int* __restrict__ entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int per_unit, float* o_part, float* ml_part,
     __nv_bfloat16* out, int* status, int early) {
     if (!early) il_pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];
@@ -174,17 +189,19 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
     // early: the caller vouches that lengths, block tables and the pages of earlier tokens do not come from the kernel in front (which writes q and
     // the newest token's slot, in the last page). What depends only on them is then done before waiting for it.
     int from, to, e, before;
-    if (whole) {                                  // one unit
+    if (per_unit) {                               // one unit, or this block's share of it
         int first;
-        e = blockIdx.x / units, before = 0;
+        const int u = blockIdx.x / per_unit, rank = blockIdx.x - u * per_unit;
+        e = u / units, before = 0;
         const int n = dq_pages(entry_kvlen[e], window, &first);
-        from = (blockIdx.x - e * units) * n, to = from + n;
+        from = (u - e * units) * n + n * rank / per_unit, to = (u - e * units) * n + n * (rank + 1) / per_unit;
     } else {
         const DqDeal d = dq_deal(entry_kvlen, n_decode, window, units, n_blocks, blockIdx.x, lane);
         e = d.e, before = d.before;
         from = min((long long)blockIdx.x * d.share, (long long)d.all), to = min((long long)from + d.share, (long long)d.all);
     }
 
+    if (per_unit > 1 && from >= to && threadIdx.x < ROWS) reinterpret_cast<float2*>(smem)[DQ_WARPS * ROWS + threadIdx.x] = make_float2(-INFINITY, 0.f);      // (no pages: no part)
     const uint32_t pipe = (uint32_t)__cvta_generic_to_shared(smem) + warp * DQ_STAGES * DQ_REC;
     const uint32_t bars = (uint32_t)__cvta_generic_to_shared(smem) + BARS + warp * DQ_STAGES * 8;
     uint2* q_sm = reinterpret_cast<uint2*>(smem + dq_q(ROWS));             // [product step][lane][NT]
@@ -483,7 +500,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
             *reinterpret_cast<float2*>(sm_ml + (DQ_WARPS * ROWS + r) * 2) = make_float2(M, L);
         }
         __syncthreads();
-        // final where the whole unit lies in this block, else a part
+        // final where the whole unit lies in this block, else a part: in scratch, or for the cluster here, in the first warp's place
         const bool final = start >= from && start + n_pages <= to;
         const size_t place = 2 * blockIdx.x + (start >= from ? 1 : 0);
         __nv_bfloat16* out_rows = out + ((size_t)e * nh + head0) * DQ_HD;
@@ -498,11 +515,35 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                 const float4 v = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * ROWS + r) * DQ_OS + d);
                 acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
             }
-            dq_write(acc, ML.x, ML.y, final ? out_rows : nullptr, o_part + place * ROWS * DQ_HD, ml_part + place * (2 * ROWS), r, d);
+            if (per_unit > 1) *reinterpret_cast<float4*>(sm_o + (size_t)r * DQ_OS + d) = acc;
+            else dq_write(acc, ML.x, ML.y, final ? out_rows : nullptr, o_part + place * ROWS * DQ_HD, ml_part + place * (2 * ROWS), r, d);
         }
         __syncthreads();                              // the next stretch's copies come where the merge was
     }
     if (!waited) il_pdl_wait();
+    if (per_unit > 1) {                           // the cluster's parts added up in block order, each block a share of the columns
+        const uint32_t sm_ml = (uint32_t)__cvta_generic_to_shared(smem) + DQ_WARPS * ROWS * 8, sm_o = sm_ml + ROWS * 8;
+        const int u = blockIdx.x / per_unit, rank = blockIdx.x - u * per_unit, i = u / units, head = (u - i * units) / row_tiles, rt = u - i * units - head * row_tiles;
+        const int head0 = head * G + rt * ROWS, rows_valid = min(ROWS, G - rt * ROWS);
+        il_cluster_sync();
+        for (int idx = rank * DQ_WARPS * 32 + threadIdx.x; idx < rows_valid * (DQ_HD / 4); idx += per_unit * DQ_WARPS * 32) {
+            const int r = idx / (DQ_HD / 4), d = (idx - r * (DQ_HD / 4)) * 4;
+            float2 ml[DQ_CLUSTER];
+            float4 v[DQ_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int p = 0; p < DQ_CLUSTER; ++p)
+                if (p < per_unit) ml[p] = dq_peer2(sm_ml + r * 8, p), v[p] = dq_peer4(sm_o + (r * DQ_OS + d) * 4, p), M = fmaxf(M, ml[p].x);
+#pragma unroll
+            for (int p = 0; p < DQ_CLUSTER; ++p)
+                if (p < per_unit && ml[p].x != -INFINITY) {           // (no part: what lies there is not one)
+                    const float f = dq_ex2(ml[p].x - M);
+                    L += f * ml[p].y, acc.x += f * v[p].x, acc.y += f * v[p].y, acc.z += f * v[p].z, acc.w += f * v[p].w;
+                }
+            dq_write(acc, M, L, out + ((size_t)i * nh + head0) * DQ_HD, nullptr, nullptr, r, d);
+        }
+        il_cluster_sync();                        // (nobody leaves while its part is read)
+    }
     // requests without a key: zeros
     for (int z = blockIdx.x; z < n_decode; z += n_blocks)
         if (entry_kvlen[z] <= 0)
@@ -630,7 +671,7 @@ IL_EXPORT int il_attn_decode_quant_resident_blocks(int group) {
     return least * sms;
 }
 
-// n_blocks: blocks that the pages are dealt out to, or 0: a block a unit. Scratch for n_blocks > 0: o_part float32 [2 * n_blocks * 16 * head_dim], ml_part [2 * n_blocks * 32].
+// n_blocks: blocks that the pages are dealt out to; 0: a block a unit; -2 .. -8: a cluster of so many blocks a unit. Scratch for n_blocks > 0: o_part float32 [2 * n_blocks * 16 * head_dim], ml_part [2 * n_blocks * 32].
 // (Arguments as one struct: see kv_quant.cu.)
 struct DqArgs {
     const void* q;
@@ -649,21 +690,27 @@ IL_EXPORT int il_attn_decode_quant(const DqArgs* args) {
     const int kind = a.kind, n_decode = a.n_decode, nh = a.nh, nkv = a.nkv, hd = a.hd, n_blocks = a.n_blocks;
     if (n_decode <= 0) return IL_OK;
     if (hd != HEAD_DIM) return IL_UNSUPPORTED;
-    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < 0 || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !a.status) return IL_BAD_ARG;
+    if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || n_blocks < -DQ_CLUSTER || (kind != KVQ_E4M3 && kind != KVQ_INT8) || !a.status) return IL_BAD_ARG;
     const int group = nh / nkv, rows = group <= 8 ? 8 : 16, row_tiles = (group + rows - 1) / rows, units = nkv * row_tiles;
-    if ((long long)n_decode * units * a.bt_stride > 0x7fffffffLL || n_blocks > 0x3fffffff) return IL_UNSUPPORTED;   // (pages of all units are counted in 32 bits)
+    if ((long long)n_decode * units * (a.bt_stride > DQ_CLUSTER ? a.bt_stride : DQ_CLUSTER) > 0x7fffffffLL || n_blocks > 0x3fffffff) return IL_UNSUPPORTED;   // (pages of all units are counted in 32 bits)
     if (n_blocks > 0 && (!a.o_part || !a.ml_part)) return IL_BAD_ARG;
     if ((((uintptr_t)a.cache | (uintptr_t)a.q | (uintptr_t)a.out) & 15) || (a.q_stride & 7) || a.q_stride < (long long)nh * hd) return IL_BAD_ARG;
     int dev = 0;
     cudaGetDevice(&dev);
     const int rc = dq_prepare(dev);
     if (rc != IL_OK) return rc;
-    const int whole = n_blocks == 0;
+    const int per_unit = n_blocks > 0 ? 0 : n_blocks == 0 ? 1 : -n_blocks;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = il_pdl_enabled();
+    attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = per_unit, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(per_unit ? n_decode * units * per_unit : n_blocks), cfg.blockDim = dim3(DQ_WARPS * 32), cfg.stream = a.stream, cfg.attrs = attr, cfg.numAttrs = per_unit > 1 ? 2 : 1;
     cudaError_t e = dq_pick(kind, group, [&](auto kernel, int smem) {
-        return il_launch(kernel, dim3(whole ? n_decode * units : n_blocks), dim3(DQ_WARPS * 32), (size_t)smem, a.stream, (const __nv_bfloat16*)a.q, a.q_stride, (const unsigned char*)a.cache, a.block_table, a.bt_stride,
-                         a.entry_kvlen, n_decode, nh, nkv, group, row_tiles, a.scale * 1.4426950408889634f, a.window, whole, a.o_part, a.ml_part, (__nv_bfloat16*)a.out, a.status, a.early);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        return cudaLaunchKernelEx(&cfg, kernel, (const __nv_bfloat16*)a.q, (long long)a.q_stride, (const unsigned char*)a.cache, a.block_table, (int)a.bt_stride, a.entry_kvlen, (int)n_decode, (int)nh,
+                                  (int)nkv, (int)group, (int)row_tiles, a.scale * 1.4426950408889634f, (int)a.window, (int)per_unit, a.o_part, a.ml_part, (__nv_bfloat16*)a.out, a.status, (int)a.early);
     });
-    if (e == cudaSuccess && !whole) {
+    if (e == cudaSuccess && !per_unit) {
         // warps a row by the parts that a unit has if the requests are alike
         const int parts = n_blocks / (n_decode * units), n_rows = n_decode * nh;
         const auto merge = [&](auto kernel, int blocks, int threads) {

@@ -1972,15 +1972,17 @@ def kv_unpack(cache: torch.Tensor, kind: str, block_table: torch.Tensor, entry_k
 
 
 _resident_quant = {}
-# A block a unit, with every sum final, where dealing the pages out would take less than so many of them off the longest block: the second kernel then costs more than it
-# saves. Dealt out / whole, us: 64 requests of 256 tokens (16 pages), 32 heads on 8 of 128, 15.8 / 9.4; of 512 19.9 / 13.9; one request of 256, 32 heads on 2, 7.5 / 7.5, of 512
-# (24 pages less) 8.6 / 10.4.
-QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES = 8, 12
+# How a unit's pages meet blocks. A block a unit, with every sum final, where dealing the pages out to one wave of blocks would take less than so many off the longest block: the second
+# kernel then costs more than it saves. Else a cluster of two to eight blocks a unit, which add their parts up themselves, while that leaves a block few enough more than dealing out does
+# (fewer with two column tiles of heads, where a page takes longer) and no more than QUANT_CLUSTER_MOST (all units count as long as the longest here). Whole / cluster / dealt out, us, heads
+# of 128: 64 requests of 256 tokens (16 pages), 32 heads on 8, 9.0 / - / 14.9; one of 256, 32 on 2, 6.7 / 6.6 / 7.4; of 512 9.3 / 6.7 / 7.8; of 1,536 - / 8.4 / 8.7; of 2,048 - / 9.3 / 8.7; three of 100, eight heads of 64, 4.3 / 5.1 / 8.9; eight
+# of 1,024, 32 on 8, - / 8.1 / 10.2; four of 2,560 - / 9.3 / 12.2; sixteen of 1,024 15.5 / 12.0 / 15.1; one of 4,096 - / 9.3 / 8.1.
+QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES, QUANT_CLUSTER_PAGES, QUANT_CLUSTER_MOST = 8, 12, (12, 6), 32
 
 
 def _quant_blocks(head_dim: int, group: int, units: int, pages: int, device: Optional[int] = None) -> int:
     """Blocks that the pages of `units` units (a kv head of a request with up to 8 or 16 of its `group` query heads) of at most `pages` pages are dealt out to: one wave of
-    them, eight pages each at least; 0: a block a unit."""
+    them, eight pages each at least; 0: a block a unit; below 0: a cluster of as many."""
     key = (_cur_device() if device is None else device, head_dim, group > 8)
     most = _resident_quant.get(key)
     if most is None:
@@ -1989,8 +1991,17 @@ def _quant_blocks(head_dim: int, group: int, units: int, pages: int, device: Opt
         most = _resident_quant[key] = int(fn(group))
         if most <= 0:
             raise KernelError("attention_decode_quant: the occupancy query failed")
-    least = QUANT_LEAST_PAGES
-    if pages <= QUANT_WHOLE_PAGES + max(least, units * pages // most):
+    least, cluster = QUANT_LEAST_PAGES, 1
+    if pages <= QUANT_WHOLE_PAGES:
+        return 0
+    share = max(least, units * pages // most)
+    # more blocks a unit: while there are few, down to a page a warp; while one wave has room, down to four pages a warp
+    while cluster < 8 and (units * 2 * cluster <= 256 and pages > 4 * cluster or units * 2 * cluster <= most and pages > 16 * cluster):
+        cluster *= 2
+    longest = (pages + cluster - 1) // cluster
+    if cluster > 1 and longest <= min(share + QUANT_CLUSTER_PAGES[group > 8], QUANT_CLUSTER_MOST):
+        return -cluster
+    if pages <= QUANT_WHOLE_PAGES + share:
         return 0
     return min(most, units * ((pages + least - 1) // least))
 

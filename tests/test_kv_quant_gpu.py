@@ -284,7 +284,7 @@ def _decode_check(out, q, val, rows, kvlens, nh, hd, scale, window):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 64), (4, 4, 64), (32, 2, 128), (6, 2, 128), (20, 1, 128), (8, 2, 256), (40, 1, 64)])
-@pytest.mark.parametrize("blocks", [0, 1, 2, 7, 300])
+@pytest.mark.parametrize("blocks", [0, 1, 2, 7, 300, -2, -4, -8])
 @pytest.mark.parametrize("window", [None, 20, -24])
 def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, window):
     ops, dev = _ops(), cuda_device
@@ -312,7 +312,7 @@ def test_decode_over_codes(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, 
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128, 256])
-@pytest.mark.parametrize("blocks", [0, 5, 23])
+@pytest.mark.parametrize("blocks", [0, 5, 23, -2, -8])
 def test_decode_pages_that_are_not_there_and_rows_that_are_not_finite(cuda_device, monkeypatch, kind, hd, blocks):
     """A missing page's keys are masked, a request without any page gets zeros; a NaN row reaches the heads and requests that see it, no others; exponents far apart."""
     ops, dev = _ops(), cuda_device
@@ -367,7 +367,7 @@ def test_decode_takes_rows_with_a_stride_and_is_repeatable(cuda_device):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("blocks", [16, 17, 100, 600])
+@pytest.mark.parametrize("blocks", [16, 17, 100, 600, -8])
 def test_decode_of_long_contexts_in_many_parts(cuda_device, monkeypatch, kind, hd, blocks):
     """Parts by the hundred of one unit, beside requests of a page; the same bits twice."""
     ops, dev = _ops(), cuda_device
@@ -677,7 +677,7 @@ def test_two_captured_steps_that_share_a_workspace(cuda_device):
     ops.check_status(dev)
 
 
-@pytest.mark.parametrize("blocks", [None, 0])
+@pytest.mark.parametrize("blocks", [None, 0, -4])
 @pytest.mark.parametrize("nh", [4, 12])
 def test_decode_of_a_thousand_requests(cuda_device, monkeypatch, blocks, nh):
     """More requests than a warp's lanes count at a time, many without a key, next to long ones."""
