@@ -14,12 +14,12 @@
 //   softmax and output of A and of B. All 512 columns of tensor memory and (head_dim 128) 192 KB of shared memory: one block an SM.
 //   What bounds it: a row tile's chain, some 3,250 clocks a key tile - its products 890, their way to the softmax and back 500, loads and maximum 450, exponentials 1,300 (1,024 of them
 //   the special-function unit's) -, two of which the block runs against each other; the tensor cores are busy seven tenths of it. One row tile a block, key tiles of 64 and two
-//   blocks an SM (attn_prefill_tc5) / this, us with the pages' reading: 8,192 tokens, 32 heads on 8 of 128, 563 / 501; 4,096 of 32 on 2 164 / 145; 8,192 of 16 on 2 of 64 265 / 209; 1,024 behind
-//   8,000, 32 on 8, 170 / 144. Slower were: a thread of its own for each row tile's products (they then interleave in the tensor cores: 728 for 501), P handed over in halves
+//   blocks an SM (attn_prefill_tc5) / this, us with the pages' reading: 8,192 tokens, 32 heads on 8 of 128, 563 / 483; 4,096 of 32 on 2 164 / 145 to 159; 8,192 of 16 on 2 of 64 265 / 209; 1,024 behind
+//   8,000, 32 on 8, 170 / 144. Slower, from 501 us of the first, were: a thread of its own for each row tile's products (they then interleave in the tensor cores: 728 for 501), P handed over in halves
 //   (492, but 152 for 145), one pair of exponentials of eight by a polynomial on the multiply-add units (549), scores read twice instead of kept in registers (512).
 //
 //   Every mbarrier wait is bounded; one that runs out sets *status and all roles leave their loops.
-//   grid (tiles, kv heads). Tiles of 2 TPT tokens are numbered over the entries [first_entry, n_entries) in order; a block finds its entry by walking entry_qstart.
+//   grid tiles x kv heads. Tiles of 2 TPT tokens are numbered over the entries [first_entry, n_entries) in order; a block finds its entry by walking entry_qstart.
 #include "tcgen05.cuh"
 
 #ifndef HEAD_DIM
@@ -80,9 +80,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) attn_prefill_pair_kernel(
         if (threadIdx.x == 0) atomicExch(status, 101);
         return;
     }
-    const int G = nh / nkv, g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // which entry and which tokens: tiles are taken from the last to the first, the longest blocks start first
-    int tile = (int)gridDim.x - 1 - (int)blockIdx.x, e = first_entry;
+    const int G = nh / nkv, g = blockIdx.x % nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Which entry and which tokens: tiles are taken from the last to the first, so that of a request the longest blocks start first, kv heads side by side (one kv head behind the other: 495 for
+    // 485 us, 8,192 tokens, 32 heads on 8 of 128; the requests by length instead: 161 for 154, five of 37 to 1,024 tokens behind up to 4,096).
+    int tile = (int)(gridDim.x / nkv - 1 - blockIdx.x / nkv), e = first_entry;
     for (; e < n_entries; ++e) {
         const int nt = (entry_qstart[e + 1] - entry_qstart[e] + 2 * tpt - 1) / (2 * tpt);
         if (tile < nt) break;
@@ -363,7 +364,7 @@ IL_EXPORT int il_attn_prefill_pair(const PpArgs* args) {
     if (hd != HEAD_DIM || !kv_map || !status) return IL_UNSUPPORTED;
     if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || first_entry < 0) return IL_BAD_ARG;
     const int G = nh / nkv;
-    if (G > PP_ROWS || !(scale > 0.f) || nkv > 65535) return IL_UNSUPPORTED;
+    if (G > PP_ROWS || !(scale > 0.f) || (long long)n_tiles_total * nkv > 0x7fffffffLL) return IL_UNSUPPORTED;
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_stride & 7)) return IL_UNSUPPORTED;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -375,7 +376,7 @@ IL_EXPORT int il_attn_prefill_pair(const PpArgs* args) {
     }
     CUtensorMap map;
     memcpy(&map, kv_map, sizeof(map));
-    attn_prefill_pair_kernel<<<dim3(n_tiles_total, nkv), PP_THREADS, PP_SMEM, stream>>>(map, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, block_table, bt_stride, entry_qstart, entry_kvlen,
+    attn_prefill_pair_kernel<<<(unsigned)(n_tiles_total * nkv), PP_THREADS, PP_SMEM, stream>>>(map, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, block_table, bt_stride, entry_qstart, entry_kvlen,
                                                                                        first_entry, n_entries, nh, nkv, scale * 1.4426950408889634f, window, PP_ROWS / G, status);
     IL_LAUNCH_CHECK();
     return IL_OK;
