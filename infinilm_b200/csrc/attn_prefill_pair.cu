@@ -41,7 +41,7 @@ constexpr int PP_PAGE_BYTES = 2 * PP_ATOM;
 constexpr int PP_K_BYTES = PP_TILE_PAGES * PP_PAGE_BYTES;
 constexpr int PP_THREADS = 384;
 constexpr int PP_COL_S = 0, PP_COL_O = 2 * PP_KEYS;           // S of A, S of B, O of A, O of B
-constexpr int PP_N_BARS = 1 + 4 * PP_STAGES + 6;
+constexpr int PP_N_BARS = 1 + 4 * PP_STAGES + 7;
 constexpr int PP_SMEM = 2 * PP_Q_BYTES + 2 * PP_STAGES * PP_K_BYTES + PP_N_BARS * 8 + 16;
 static_assert(PP_SMEM <= 227 * 1024, "shared memory of a block");
 constexpr unsigned PP_SPIN = 1u << 22;
@@ -109,9 +109,11 @@ __global__ void __launch_bounds__(PP_THREADS, 1) attn_prefill_pair_kernel(
     const uint32_t s_full0 = v_empty0 + 8 * PP_STAGES;                // a row tile's scores are complete, and so is all that O got before (tcgen05.commit)
     const uint32_t p_full0 = s_full0 + 16;                            // a row tile's P is in tensor memory (4 warps), and the keys and values that are needed next in shared memory (warp 3)
     const uint32_t o_done0 = p_full0 + 16;                            // a row tile's last product is through (tcgen05.commit)
+    const uint32_t drained = o_done0 + 16;                            // after a wait that ran out: all products are (tcgen05.commit)
     if (threadIdx.x == 0) {
         t5_mbar_init(q_full, 8);
         for (int s = 0; s < PP_STAGES; ++s) t5_mbar_init(k_full0 + 8 * s, 1), t5_mbar_init(k_empty0 + 8 * s, 1), t5_mbar_init(v_full0 + 8 * s, 1), t5_mbar_init(v_empty0 + 8 * s, 1);
+        t5_mbar_init(drained, 1);
         for (int t = 0; t < 2; ++t) t5_mbar_init(s_full0 + 8 * t, 1), t5_mbar_init(p_full0 + 8 * t, 5), t5_mbar_init(o_done0 + 8 * t, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -154,9 +156,14 @@ __global__ void __launch_bounds__(PP_THREADS, 1) attn_prefill_pair_kernel(
             return ok != 0;
         };
         bool ok = issue(0, 0);
+        int n_k = ok, n_v = 0;
         for (int j = 0; j < n_tiles && ok; ++j) {
-            if (j + 1 < n_tiles) ok = issue(j + 1, 0);
-            if (ok) ok = issue(j, 1);
+            if (j + 1 < n_tiles) ok = issue(j + 1, 0), n_k += ok;
+            if (ok) ok = issue(j, 1), n_v += ok;
+        }
+        if (lane == 0) {                          // (whatever became of the other roles: no copy may come behind the block's end)
+            for (int j = max(n_k - PP_STAGES, 0); j < n_k; ++j) t5_mbar_wait(k_full0 + 8 * (j % PP_STAGES), (uint32_t)(j / PP_STAGES) & 1u, PP_SPIN);
+            for (int j = max(n_v - PP_STAGES, 0); j < n_v; ++j) t5_mbar_wait(v_full0 + 8 * (j % PP_STAGES), (uint32_t)(j / PP_STAGES) & 1u, PP_SPIN);
         }
     } else if (warp == 2) {
         // ---------------- the tensor cores' products, one thread ----------------
@@ -198,6 +205,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) attn_prefill_pair_kernel(
                 t5_commit(v_empty0 + 8 * sv);
                 if (j + 1 < n_tiles) t5_commit(k_empty0 + 8 * sk);
             }
+            if (!ok) t5_commit(drained), t5_mbar_wait(drained, 0, PP_SPIN);        // (no product may come behind the tensor memory's release)
         }
     } else if (warp == 3) {
         // ---------------- waits for K and V on behalf of the thread that issues: its arrival at P's barriers says that V(j) and K(j + 1) are there, too. (A wait costs a thread some
