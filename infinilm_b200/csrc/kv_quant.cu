@@ -280,48 +280,24 @@ __device__ __forceinline__ int kvu_seen(const int* entry_kvlen, const int* entry
     return max(min((kvlen + KVQ_PAGE - 1) / KVQ_PAGE, width) - *first, 0);
 }
 
-// A block a page of a request. room > 0: the pages that are seen lie one behind the other, request after request, up to `room` of them, and `table` says where (0 for the others: in bounds for who looks all the same; pages for
-// which no room is left set *status); else page p of the i-th request lies at i * width + p. Pages in front of the one that holds the lowest position the request's portion sees (its first new token's, by the mask) and behind the last
-// are left as they are, slots behind the request's end become zeros. A thread makes 16 bytes of output at a time, KVU_AHEAD of them at once: bound by memory, what matters is loads under
-// way and few instructions between them. HD 0: any head size. 16 requests of up to 8,192 tokens, 8 kv heads of 128, e4m3 to bfloat16, us: 79.9 with places worked out for each piece,
-// 71.0 so (6.0 TB/s); two pieces at a time 77, eight 69.9 (but more for few tokens), sixteen 81.
-constexpr int KVU_AHEAD = 4;
+// A block a page of a request. room > 0: the pages that are seen lie one behind the other, request after request, up to `room` of them, and `table` says where (0 for the others: in bounds
+// for who looks all the same; pages for which no room is left set *status); else page p of the i-th request lies at i * width + p. Pages in front of the one that holds the lowest position
+// the request's portion sees (its first new token's, by the mask) and behind the last are left as they are, slots behind the request's end become zeros. A thread makes 16 bytes of output at a
+// time, KVU_AHEAD of them at once: bound by memory, what matters is loads under way and few instructions between them. HD 0: any head size. 16 requests of up to 8,192 tokens, 8 kv heads of
+// 128, e4m3 to bfloat16, us: 79.9 with places worked out for each piece, 71.0 so (6.0 TB/s); two pieces at a time 77, eight 69.9 (but more for few tokens), sixteen 81.
+// Dealt out (below) they take 76; but 64 requests of 300 tokens with tables of 2,048 pages 26 for 187, one of 32,000 among them 58 for 216: a block that finds nothing costs a nanosecond,
+// so tables of up to KVU_EACH pages together have a block a page.
+constexpr int KVU_AHEAD = 4, KVU_EACH = 8192, KVU_BLOCKS = 148 * 16;
 __device__ __forceinline__ void kvq_put4(float* o, float a, float b, float c, float d) { o[0] = a, o[1] = b, o[2] = c, o[3] = d; }
 __device__ __forceinline__ void kvq_put4(__nv_bfloat16* o, float a, float b, float c, float d) {
     *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(a, b), *reinterpret_cast<__nv_bfloat162*>(o + 2) = __floats2bfloat162_rn(c, d);
 }
+// One page: its records to the rows of `out`.
 template <typename TO, int KIND, int HD>
-__global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
-                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room, int* status) {
-    il_pdl_begin();
-    constexpr int VEC = 16 / sizeof(TO);
+__device__ __forceinline__ void kvu_page(const unsigned char* recs, TO* out, int n_keys, int nkv, int hd_arg, int told_by_key) {
     const int hd = HD ? HD : hd_arg;
-    const int i = blockIdx.y, e = first_entry + i, p = blockIdx.x;
-    int first;
-    const int n_seen = kvu_seen(entry_kvlen, entry_qstart, window, e, gridDim.x, &first), kvlen = entry_kvlen[e];
-    const bool seen = p >= first && p - first < n_seen;
-    size_t to = (size_t)i * gridDim.x + p;
-    if (room > 0 && seen) {                       // behind the pages of the requests in front
-        __shared__ int sums[8];
-        int sum = 0, f;
-        for (int k = threadIdx.x; k < i; k += 256) sum += kvu_seen(entry_kvlen, entry_qstart, window, first_entry + k, gridDim.x, &f);
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
-        __syncthreads();
-        sum = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum += sums[k];
-        to = (size_t)sum + (p - first);
-    }
-    const bool fits = room <= 0 || to < (size_t)room;
-    if (threadIdx.x == 0) {
-        if (table) table[(size_t)e * gridDim.x + p] = room > 0 && !(seen && fits) ? 0 : (int)to;
-        if (seen && !fits) atomicExch(status, 92);
-    }
-    if (!seen || !fits) return;
-    const int page = block_table[(size_t)e * bt_stride + p], rec_bytes = kvq_record(hd), n_keys = page < 0 ? 0 : min(KVQ_PAGE, kvlen - p * KVQ_PAGE);
-    const unsigned char* recs = cache + (size_t)max(page, 0) * nkv * rec_bytes;
-    TO* out = pages + to * 2 * nkv * KVQ_PAGE * hd;
+    constexpr int VEC = 16 / sizeof(TO);
+    const int rec_bytes = kvq_record(hd);
     const int per = hd / VEC, plane = KVQ_PAGE * per;         // pieces of a row and of a head
     // A thread has the same piece of one head after another: what it needs of the key and the column is made once. Small heads are several at a time.
     const bool several = 256 % plane == 0;
@@ -372,6 +348,99 @@ __global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* 
     }
 }
 
+template <typename TO, int KIND, int HD>
+__global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
+                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room, int* status) {
+    il_pdl_begin();
+    const int hd = HD ? HD : hd_arg;
+    const int i = blockIdx.y, e = first_entry + i, p = blockIdx.x;
+    int first;
+    const int n_seen = kvu_seen(entry_kvlen, entry_qstart, window, e, gridDim.x, &first), kvlen = entry_kvlen[e];
+    const bool seen = p >= first && p - first < n_seen;
+    size_t to = (size_t)i * gridDim.x + p;
+    if (room > 0 && seen) {                       // behind the pages of the requests in front
+        __shared__ int sums[8];
+        int sum = 0, f;
+        for (int k = threadIdx.x; k < i; k += 256) sum += kvu_seen(entry_kvlen, entry_qstart, window, first_entry + k, gridDim.x, &f);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += sums[k];
+        to = (size_t)sum + (p - first);
+    }
+    const bool fits = room <= 0 || to < (size_t)room;
+    if (threadIdx.x == 0) {
+        if (table) table[(size_t)e * gridDim.x + p] = room > 0 && !(seen && fits) ? 0 : (int)to;
+        if (seen && !fits) atomicExch(status, 92);
+    }
+    if (!seen || !fits) return;
+    const int page = block_table[(size_t)e * bt_stride + p], rec_bytes = kvq_record(hd), n_keys = page < 0 ? 0 : min(KVQ_PAGE, kvlen - p * KVQ_PAGE);
+    kvu_page<TO, KIND, HD>(cache + (size_t)max(page, 0) * nkv * rec_bytes, pages + to * 2 * nkv * KVQ_PAGE * hd, n_keys, nkv, hd, told_by_key);
+}
+
+// The same where tables are so wide, for so many requests, that most blocks of a page each might find nothing: the pages that are seen dealt out to KVU_BLOCKS blocks.
+template <typename TO, int KIND, int HD>
+__global__ void __launch_bounds__(256, 4) kv_unpack_dealt_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
+                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int n, int width, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room,
+                                                        int* status) {
+    il_pdl_begin();
+    const int hd = HD ? HD : hd_arg;
+    const int lane = threadIdx.x & 31, rec_bytes = kvq_record(hd);
+    // how many pages are seen, and the request that this block's first one belongs to, with how many lie in front of that request's (every warp for itself, a lane a request)
+    int first, all = 0, n0 = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int seen = i0 + lane < n ? kvu_seen(entry_kvlen, entry_qstart, window, first_entry + i0 + lane, width, &first) : 0;
+        if (i0 == 0) n0 = seen;
+        all += __reduce_add_sync(0xffffffffu, seen);
+    }
+    const int share = (int)(((unsigned)all + gridDim.x - 1) / gridDim.x);
+    const long long from = (long long)blockIdx.x * share;
+    if (from < all) {
+        int i = 0, before = 0;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int seen = i0 == 0 ? n0 : i0 + lane < n ? kvu_seen(entry_kvlen, entry_qstart, window, first_entry + i0 + lane, width, &first) : 0;
+            int sum = seen;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + sum > (int)from);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                i = i0 + l, before += __shfl_sync(0xffffffffu, sum - seen, l);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        int n_seen = kvu_seen(entry_kvlen, entry_qstart, window, first_entry + i, width, &first), kvlen = entry_kvlen[first_entry + i];
+        for (int at = (int)from; at < min(from + share, (long long)all); ++at) {
+            while (at >= before + n_seen) {
+                before += n_seen, ++i;
+                n_seen = kvu_seen(entry_kvlen, entry_qstart, window, first_entry + i, width, &first), kvlen = entry_kvlen[first_entry + i];
+            }
+            if (room > 0 && at >= room) {
+                if (threadIdx.x == 0) atomicExch(status, 92);
+                break;
+            }
+            const int p = first + at - before, page = block_table[(size_t)(first_entry + i) * bt_stride + p], n_keys = page < 0 ? 0 : min(KVQ_PAGE, kvlen - p * KVQ_PAGE);
+            const size_t to = room > 0 ? at : (size_t)i * width + p;
+            kvu_page<TO, KIND, HD>(cache + (size_t)max(page, 0) * nkv * rec_bytes, pages + to * 2 * nkv * KVQ_PAGE * hd, n_keys, nkv, hd, told_by_key);
+        }
+    }
+    if (table)
+        for (int i = blockIdx.x; i < n; i += gridDim.x) {
+            int before = 0;
+            for (int k = lane; k < i; k += 32) before += kvu_seen(entry_kvlen, entry_qstart, window, first_entry + k, width, &first);
+            before = __reduce_add_sync(0xffffffffu, before);
+            const int n_seen = kvu_seen(entry_kvlen, entry_qstart, window, first_entry + i, width, &first), n_fit = min(n_seen, max(room - before, 0));
+            for (int p = threadIdx.x; p < width; p += 256)
+                table[(size_t)(first_entry + i) * width + p] = room <= 0 ? i * width + p : p >= first && p - first < n_fit ? before + p - first : 0;
+        }
+}
+
 struct KvqUnpackArgs {
     const void* cache;
     const int *block_table, *entry_kvlen, *entry_qstart;
@@ -391,9 +460,16 @@ IL_EXPORT int il_kv_unpack(const KvqUnpackArgs* args) {
     if ((long long)n * width > 0x7fffffffLL) return IL_UNSUPPORTED;
     if (room < 0 || (room > 0 && (!table || !status))) return IL_BAD_ARG;
     if ((kind != KVQ_E4M3 && kind != KVQ_INT8) || (out_kind != IL_F32 && out_kind != IL_BF16)) return IL_BAD_ARG;
-#define KVU_OF(TO, KIND, HD)                                                                                                                                \
-    IL_LAUNCH((kv_unpack_kernel<TO, KIND, HD>), dim3(width, n), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen, entry_qstart, \
-              window, first_entry, nkv, hd, (TO*)pages, table, told_by_key, room, status)
+    const bool each = (long long)n * width <= KVU_EACH;
+#define KVU_OF(TO, KIND, HD)                                                                                                                                     \
+    do {                                                                                                                                                         \
+        if (each)                                                                                                                                                \
+            IL_LAUNCH((kv_unpack_kernel<TO, KIND, HD>), dim3(width, n), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen,        \
+                      entry_qstart, window, first_entry, nkv, hd, (TO*)pages, table, told_by_key, room, status);                                                 \
+        else                                                                                                                                                     \
+            IL_LAUNCH((kv_unpack_dealt_kernel<TO, KIND, HD>), dim3(KVU_BLOCKS), 256, 0, stream, (const unsigned char*)cache, block_table, bt_stride, entry_kvlen, \
+                      entry_qstart, window, first_entry, n, width, nkv, hd, (TO*)pages, table, told_by_key, room, status);                                       \
+    } while (0)
 #define KVU_GO(TO, KIND)                                 \
     do {                                                 \
         if (hd == 64) KVU_OF(TO, KIND, 64);              \

@@ -272,6 +272,47 @@ def test_unpack_packed(cuda_device, kind, n):
             ops.check_status(dev)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,dtype", [(16, torch.bfloat16), (64, torch.float32), (128, torch.bfloat16)])
+@pytest.mark.parametrize("window", [None, 20, -32])
+def test_unpack_with_wide_tables(cuda_device, kind, hd, dtype, window):
+    """Many requests with tables far wider than they need (the pages are then dealt out to blocks): what narrow tables give, packed and by place."""
+    ops, dev = _ops(), cuda_device
+    n, nkv, narrow, wide = 300, 2, 6, 40
+    g = torch.Generator().manual_seed(hd)
+    kvlens = [0 if i % 5 == 2 else int(torch.randint(0, 90, (1,), generator=g)) for i in range(n)]
+    kvlens[0], kvlens[299] = 96, 95
+    new = [min(k, 1 + i % 3) for i, k in enumerate(kvlens)]
+    qs = [0]
+    for x in new:
+        qs.append(qs[-1] + x)
+    rows, n_pages = _tables(kvlens, 0, 21, width=narrow)
+    cache = _cache(n_pages, nkv, hd, kind, 22)[0].to(dev)
+    rest = dict(entry_kvlen=_i32(kvlens, dev), entry_qstart=_i32(qs, dev), window=window)
+    got = []
+    for width in (narrow, wide):
+        tab = _i32([r + [-1] * (width - narrow) for r in rows], dev)
+        for first in (0, 7):
+            pages, table = torch.full((n_pages, 2, nkv, 16, hd), 77.0, dtype=dtype, device=dev), torch.full_like(tab, -5)
+            ops.kv_unpack(cache, kind, tab, pages=pages, table=table, first_entry=first, packed=True, **rest)
+            placed, by_place = torch.full((n * width, 2, nkv, 16, hd), 77.0, dtype=dtype, device=dev), torch.full_like(tab, -5)
+            ops.kv_unpack(cache, kind, tab, pages=placed, table=by_place, first_entry=first, **rest)
+            assert not table[first:, narrow:].any() and (table[:first] == -5).all() and (by_place[:first] == -5).all()
+            assert torch.equal(by_place[first:].cpu(), torch.arange((n - first) * width, dtype=torch.int32).view(n - first, width))
+            spare = placed[(n - first) * width:]
+            assert (spare == 77.0).all() and (placed[:(n - first) * width].view(n - first, width, -1)[:, narrow:] == 77.0).all()
+            got.append((pages, table[first:, :narrow], placed[:(n - first) * width].view(n - first, width, -1)[:, :narrow]))
+    for a, b in ((0, 2), (1, 3)):
+        assert all(torch.equal(x, y) for x, y in zip(got[a], got[b]))
+    ops.check_status(dev)
+    few = torch.full((5, 2, nkv, 16, hd), 77.0, dtype=dtype, device=dev)
+    table = torch.full_like(tab, -5)
+    ops.kv_unpack(cache, kind, tab, pages=few[:4], table=table, packed=True, **rest)
+    assert torch.equal(few[:4], got[0][0][:4]) and (few[4] == 77.0).all() and int(table.max()) == 3
+    with pytest.raises(ops.KernelError, match="kv_quant"):
+        ops.check_status(dev)
+
+
 # ---- single tokens -----------------------------------------------------------------------------------------------------------
 def _decode_check(out, q, val, rows, kvlens, nh, hd, scale, window):
     for e, n in enumerate(kvlens):
