@@ -27,6 +27,8 @@
 // Token t (= entry t) sits at position kvlen - 1 and sees positions max(0, kvlen - window) .. kvlen - 1 (window < 0: runs of -window; 0: all). No
 // key to see: zeros. A block-table entry below 0 is never followed, its keys count as masked. A masked key's score is replaced and its codes of V cleared, so
 // what a page holds behind a request's end does not matter.
+#include <cfloat>
+
 #include "kv_quant.cuh"
 
 #ifndef HEAD_DIM
@@ -63,6 +65,11 @@ __device__ __forceinline__ void dq_mma(float (&d)[4], const uint32_t (&a)[4], ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void dq_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {       // sums from zero
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Four codes of a word as two pairs of halves. e4m3: bytes 0 and 1, then 2 and 3, by the conversion instruction (shifts and masks instead, which run on another
 // unit, were slower for K, for V and for both: 112, 112 and 123 us where this takes 108, 64 requests of up to 8,192 tokens, 32 heads on 8 of 128). Whole numbers: bytes 0 and 2, then 1 and 3; 1024 + 128 +
@@ -301,7 +308,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
         float m[NT][2];
         il_f2 l[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -INFINITY, l[j] = il_f2_dup(0.f);
+        for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -FLT_MAX, l[j] = il_f2_dup(0.f);
         for (int it = 0; it < n_my; ++it) {
             if (!dq_wait(bars + (done + it) % DQ_STAGES * 8, (done + it) / DQ_STAGES & 1)) {
                 if (lane == 0) atomicExch(status, 91);
@@ -309,13 +316,9 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                 dead = true;
                 break;
             }
-            const unsigned char* rec = smem + (size_t)(warp * DQ_STAGES + (done + it) % DQ_STAGES) * DQ_REC;
+            unsigned char* rec = smem + (size_t)(warp * DQ_STAGES + (done + it) % DQ_STAGES) * DQ_REC;
             // ---- scores of the page's 16 keys: elements 0, 1 are key lg and heads 8 j + 2 lq, + 1; elements 2, 3 key 8 + lg
-            float s[NT][4], s1[NT][4];            // (two chains of products: one is all latency)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[j][i] = s1[j][i] = 0.f;
+            float s[NT][4], s1[NT][4];            // (two chains of products where there is one column tile: one alone is all latency)
 #pragma unroll
             for (int kg = 0; kg < DQ_KG; ++kg) {
                 uint32_t c[2][4];
@@ -338,19 +341,21 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                         qf[0] = q_sm[(4 * kg + i) * 32 + lane];
                     }
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) dq_mma(i & 1 ? s1[j] : s[j], a, qf[j].x, qf[j].y);
+                    for (int j = 0; j < NT; ++j) {
+                        float(&sum)[4] = NT == 1 && (i & 1) ? s1[j] : s[j];
+                        if (kg == 0 && i < (NT == 1 ? 2 : 1)) dq_mma_first(sum, a, qf[j].x, qf[j].y);
+                        else dq_mma(sum, a, qf[j].x, qf[j].y);
+                    }
                 }
             }
+            if constexpr (NT == 1)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[j][i] += s1[j][i];
+                for (int i = 0; i < 4; ++i) s[0][i] += s1[0][i];
             // ---- exponents of this lane's two keys, softmax in base 2, two heads an instruction. K's power and V's inverse power are made one unit of 2^-23 too large,
             // so that the byte of a row that is NaN, 255, gives a NaN and not an infinity.
             const int page0 = (p0 + warp + it * DQ_WARPS) * KVQ_PAGE;
             const bool gone = (bad >> (it & 31)) & 1, edge = gone || page0 < lo || page0 + KVQ_PAGE > kvlen;
             float tv[NT][4], inv_v[2];
-            uint32_t seen[2] = {0u, 0u};          // on a page that is not seen whole: the bytes of V's pairs of keys 2 lq, + 1 and 8 + 2 lq, + 1 that count (e4m3 has codes that are NaN)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const uint32_t ke = rec[2 * KVQ_PAGE * DQ_HD + 8 * n + lg], ve = rec[2 * KVQ_PAGE * DQ_HD + KVQ_PAGE + 8 * n + lg];
@@ -361,13 +366,14 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                     il_f2_get(il_f2_fma(il_f2_mul(il_f2_make(s[j][2 * n], s[j][2 * n + 1]), il_f2_dup(kp)), s_scale[j], il_f2_dup(add)), tv[j][2 * n], tv[j][2 * n + 1]);
             }
             if (edge) {
+                if (KIND == KVQ_E4M3)             // (which has codes that are NaN: rows of V that do not count are cleared where they lie)
+                    for (int i = lane; i < KVQ_PAGE * DQ_CH; i += 32) {
+                        const int k = i / DQ_CH, key = page0 + k;
+                        if (gone || key < lo || key >= kvlen) *reinterpret_cast<uint4*>(rec + KVQ_PAGE * DQ_HD + (i ^ kvq_turn(DQ_HD, true, k)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                __syncwarp();
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int key = page0 + 8 * n + 2 * lq + j;
-                        if (!gone && key >= lo && key < kvlen) seen[n] |= j ? 0xff00ff00u : 0x00ff00ffu;
-                    }
                     const int key = page0 + 8 * n + lg;
                     if (gone || key < lo || key >= kvlen) {
                         inv_v[n] = 0.f;
@@ -376,10 +382,18 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                     }
                 }
             }
-            bool up = false;
+            // how far above the maximum (which starts at the lowest float, so that no difference is one of infinities)
+            float dv[NT][4], top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) up |= fmaxf(tv[j][0], tv[j][2]) > m[j][0] + DQ_RAISE || fmaxf(tv[j][1], tv[j][3]) > m[j][1] + DQ_RAISE;
-            if (__any_sync(0xffffffffu, up)) {    // also the first keys of a head (m = -inf)
+            for (int j = 0; j < NT; ++j) {
+                const il_f2 neg_m = il_f2_make(-m[j][0], -m[j][1]);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    il_f2_get(il_f2_add(il_f2_make(tv[j][2 * n], tv[j][2 * n + 1]), neg_m), dv[j][2 * n], dv[j][2 * n + 1]);
+                    top = fmaxf(fmaxf(top, dv[j][2 * n]), dv[j][2 * n + 1]);
+                }
+            }
+            if (__any_sync(0xffffffffu, top > DQ_RAISE)) {           // also the first keys of a head
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float corr[2];
@@ -389,8 +403,8 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                         const float mn = mx > m[j][i] + DQ_RAISE ? mx : m[j][i];
-                        corr[i] = mn == m[j][i] ? 1.f : dq_ex2(m[j][i] - mn);     // 0 when nothing was summed yet
-                        m[j][i] = mn;
+                        corr[i] = dq_ex2(m[j][i] - mn);           // 0 when nothing was summed yet
+                        m[j][i] = mn, dv[j][i] = tv[j][i] - mn, dv[j][2 + i] = tv[j][2 + i] - mn;
                     }
                     l[j] = il_f2_mul(l[j], il_f2_make(corr[0], corr[1]));
 #pragma unroll
@@ -400,10 +414,9 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
             uint32_t pf[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const float m0 = m[j][0] == -INFINITY ? 0.f : m[j][0], m1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const float w0 = dq_ex2(tv[j][2 * n] - m0), w1 = dq_ex2(tv[j][2 * n + 1] - m1);
+                    const float w0 = dq_ex2(dv[j][2 * n]), w1 = dq_ex2(dv[j][2 * n + 1]);
                     l[j] = il_f2_fma(il_f2_make(w0, w1), il_f2_dup(inv_v[n]), l[j]);          // (this lane's keys; a head's lanes are added at the end)
                     pf[j][n] = dq_transpose(dq_pack_half(w0, w1));
                 }
@@ -432,8 +445,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quan
                         uint32_t a[4];
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
-                            uint32_t w = __byte_perm(x[2 * n][i], x[2 * n + 1][i], KIND == KVQ_E4M3 ? (c ? 0x7362 : 0x5140) : (c ? 0x7632 : 0x5410));
-                            if (KIND == KVQ_E4M3 && edge) w &= seen[n];
+                            const uint32_t w = __byte_perm(x[2 * n][i], x[2 * n + 1][i], KIND == KVQ_E4M3 ? (c ? 0x7362 : 0x5140) : (c ? 0x7632 : 0x5410));
                             dq_halves<KIND>(w, a[2 * n], a[2 * n + 1]);
                         }
 #pragma unroll
