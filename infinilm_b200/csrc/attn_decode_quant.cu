@@ -56,8 +56,9 @@ __host__ __device__ constexpr int dq_bars(int rows) {
 }
 __host__ __device__ constexpr int dq_q(int rows) { return dq_bars(rows) + (DQ_WARPS * DQ_STAGES * 8 + 15) / 16 * 16; }          // q's halves and the heads' factors
 __host__ __device__ constexpr int dq_smem(int rows) { return dq_q(rows) + rows * DQ_HD * 2 + rows * 4; }
-// Blocks an SM that the registers are to allow.
-constexpr int dq_per_sm(int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? 4 : (nt == 1 ? 3 : 2); }
+// Blocks an SM that the registers are to allow. (Heads of 128, three / four, us: 64 requests of up to 8,192 tokens, 32 heads on 8, e4m3, 107.5 / 106.0; 32 of 4,096, 32 on 2, e4m3, 20.8 / 19.4; one of
+// 131,072, whole numbers, whose codes take more registers to convert, 22.1 / 24.8. Five spill: 29 to 30 for the last two.)
+constexpr int dq_per_sm(int kind, int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 2 && kind == KVQ_INT8 ? 3 : 4) : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
 constexpr float DQ_RAISE = 8.f;                   // the running maximum follows only when a page's is more than this above it (log2 units)
 
@@ -183,7 +184,7 @@ __device__ __forceinline__ void dq_write(const float4& acc, float M, float L, __
 // (q and the newest token's slot of the cache, and in the second kernel the parts, are written by the kernel before and read after a wait that is not the
 // kernel's first statement: they are not declared __restrict__.)
 template <int KIND, int NT>
-__global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(NT)) attn_decode_quant_kernel(
+__global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decode_quant_kernel(
     const __nv_bfloat16* q, long long q_stride, const unsigned char* cache, const int* __restrict__ block_table, int bt_stride,
     const int* __restrict__ entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int per_unit, float* o_part, float* ml_part,
     __nv_bfloat16* out, int* status, int early) {
@@ -670,17 +671,13 @@ static int dq_prepare(int dev) {
     return IL_OK;
 }
 
-// Blocks that this device runs at once, of either kind of cache, with `group` query heads a kv head; 0 if the query fails.
-IL_EXPORT int il_attn_decode_quant_resident_blocks(int group) {
-    int dev = 0, sms = 0, least = 1 << 20;
-    if (cudaGetDevice(&dev) != cudaSuccess || dq_prepare(dev) != IL_OK || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) least = 0;
-    for (int kind = 0; kind < 2 && least; ++kind) {
-        int n = 0;
-        if (dq_pick(kind, group, [&](auto kernel, int smem) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, DQ_WARPS * 32, smem); }) != cudaSuccess) n = 0;
-        least = n < least ? n : least;
-    }
-    if (!least) cudaGetLastError();
-    return least * sms;
+// Blocks that this device runs at once, with `group` query heads a kv head; 0 if the query fails.
+IL_EXPORT int il_attn_decode_quant_resident_blocks(int kind, int group) {
+    int dev = 0, sms = 0, n = 0;
+    const bool ok = cudaGetDevice(&dev) == cudaSuccess && dq_prepare(dev) == IL_OK && cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+                    dq_pick(kind, group, [&](auto kernel, int smem) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, DQ_WARPS * 32, smem); }) == cudaSuccess;
+    if (!ok) cudaGetLastError();
+    return ok ? n * sms : 0;
 }
 
 // n_blocks: blocks that the pages are dealt out to; 0: a block a unit; -2 .. -8: a cluster of so many blocks a unit. Scratch for n_blocks > 0: o_part float32 [2 * n_blocks * 16 * head_dim], ml_part [2 * n_blocks * 32].

@@ -1981,15 +1981,15 @@ _resident_quant = {}
 QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES, QUANT_WHOLE_MOST, QUANT_CLUSTER_PAGES, QUANT_CLUSTER_MOST = 8, 12, 128, (12, 6), 32
 
 
-def _quant_blocks(head_dim: int, group: int, units: int, pages: int, device: Optional[int] = None) -> int:
+def _quant_blocks(kind: int, head_dim: int, group: int, units: int, pages: int, device: int) -> int:
     """Blocks that the pages of `units` units (a kv head of a request with up to 8 or 16 of its `group` query heads) of at most `pages` pages are dealt out to: one wave of
     them, eight pages each at least; 0: a block a unit; below 0: a cluster of as many."""
-    key = (_cur_device() if device is None else device, head_dim, group > 8)
+    key = (device, kind, head_dim, group > 8)
     most = _resident_quant.get(key)
     if most is None:
         fn = build.load("attn_decode_quant", {"HEAD_DIM": head_dim}).il_attn_decode_quant_resident_blocks
-        fn.argtypes, fn.restype = [_c_int], _c_int
-        most = _resident_quant[key] = int(fn(group))
+        fn.argtypes, fn.restype = [_c_int, _c_int], _c_int
+        most = _resident_quant[key] = int(fn(kind, group))
         if most <= 0:
             raise KernelError("attention_decode_quant: the occupancy query failed")
     least, cluster = QUANT_LEAST_PAGES, 1
@@ -2035,7 +2035,7 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     if w:
         seen = min(seen, abs(w) + KV_QUANT_PAGE)  # (a window may begin inside a page)
     group = n_heads // n_kv_heads
-    n_blocks = _quant_blocks(head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE), d)
+    n_blocks = _quant_blocks(k, head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE), d)
     parts = n_blocks > 0
     f = _quant_fns.get(("il_attn_decode_quant", head_dim)) or _quant_fn("il_attn_decode_quant", "attn_decode_quant", head_dim)
     _check(f(_packed(_DECODE_ARGS, what, q.data_ptr(), strides[0], out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(),
