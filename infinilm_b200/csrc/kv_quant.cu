@@ -50,7 +50,7 @@ __device__ __forceinline__ uint2 kvq_codes8(const float (&x)[8], float f) {
 // head, so its eight angles are made once; the lanes of a warp that need the same ones make them together. One pass, each element read once and written once; bound by
 // memory, so what matters is loads under way: the next round's while one is worked on, no barrier, registers for four blocks an SM (more rounds ahead with fewer blocks: 65 to 78 us for
 // what takes 61). `wpt`: warps a token, many where the tokens are few. 9,420 tokens, 32 heads on 8 of
-// 128, bfloat16, us: 230 with a column a lane at a time, 103 with a block a token and its angles in shared memory, 43 so.
+// 128, bfloat16, us: 230 with a column a lane at a time, 103 with a block a token and its angles in shared memory, 43 so, 40 with two columns rotated an instruction.
 constexpr int KVS_AHEAD = 1, KVS_WARPS = 148 * 16;
 template <typename TA, int KIND, int PER>
 __global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* __restrict__ tok_pos,
