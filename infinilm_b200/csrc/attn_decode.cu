@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(AD_WARPS * 32) attn_decode_kernel(
     const float* __restrict__ dist_bias, int dist_far, float cap_log2) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    // Lengths, block tables and the pages of earlier tokens do not come from the kernel before this one (it writes q and
-    // the newest token's slot in the last page): what depends only on them is done before waiting for that kernel.
+    // Launched programmatically only where the caller vouches that lengths, block tables and the pages of earlier tokens do not come from the kernel
+    // before this one (it writes q and the newest token's slot in the last page): what depends only on them is done before waiting for that kernel.
     const int split = blockIdx.x;
     const int G = nh / nkv;
     const int row_tiles = (G + 15) / 16;
@@ -524,7 +524,7 @@ static int ad_launch(const void* qkv, int row_stride, void* out, const void* cac
                      const int* entry_kvlen, int n_decode, int nh, int nkv, float scale, int window, int pages_per_split,
                      int n_splits, float* o_part, float* ml_part, cudaStream_t stream, const CUtensorMap* kv_map = nullptr,
                      int* status = nullptr, const float* sink = nullptr, int v_is_k = 0, const float* dist_bias = nullptr,
-                     int dist_far = 0, int sigmoid = 0, float cap = 0.f) {
+                     int dist_far = 0, int sigmoid = 0, float cap = 0.f, int early = 0) {
     static CUtensorMap no_map;                    // passed when there is no map: the kernel does not look at it
     int use_tma = (AD_TMA_OK && kv_map && status) ? 1 : 0;
     auto filled = [&](int i) {                    // maps behind the first are all zero where the driver did not take them
@@ -549,8 +549,9 @@ static int ad_launch(const void* qkv, int row_stride, void* out, const void* cac
     }
     const int G = nh / nkv, row_tiles = (G + 15) / 16;
     dim3 grid(n_splits, nkv * row_tiles, n_decode);
+    cudaError_t err = cudaSuccess;
 #define AD_GO(SIG, CAP)                                                                                                                      \
-    IL_LAUNCH((attn_decode_kernel<SIG, CAP>), grid, AD_WARPS * 32, smem_bytes, stream, (const __nv_bfloat16*)qkv, row_stride,                       \
+    err = il_launch_as(early != 0, attn_decode_kernel<SIG, CAP>, grid, dim3(AD_WARPS * 32), (size_t)smem_bytes, stream, (const __nv_bfloat16*)qkv, row_stride, \
               (const __nv_bfloat16*)cache, block_table, bt_stride, entry_kvlen, nh, nkv, k_scale, window, pages_per_split,               \
               n_splits, o_part, ml_part, use_tma ? *kv_map : no_map, page_map, use_tma, status,                                              \
               n_splits == 1 ? (__nv_bfloat16*)out : (__nv_bfloat16*)nullptr, sink, dist_bias, dist_far, cap * 1.4426950408889634f)
@@ -560,6 +561,7 @@ static int ad_launch(const void* qkv, int row_stride, void* out, const void* cac
     else if (cap > 0.f) AD_GO(false, true);
     else AD_GO(false, false);
 #undef AD_GO
+    if (err != cudaSuccess) return 1000 + (int)err;
     if (n_splits == 1) {                          // every row is final as the attention kernel leaves it: no merge
         IL_LAUNCH_CHECK();
         return IL_OK;
@@ -600,11 +602,12 @@ IL_EXPORT int il_attn_decode_resident_blocks_shared() { return ad_resident_block
 
 // Scratch the caller provides: o_part float32 [n_decode * nh * n_splits * head_dim], ml_part [n_decode * nh * n_splits * 2].
 // v_is_k != 0: the caller vouches that the cache's V plane repeats its K plane; with the fourth tensor map only K is read.
+// early != 0: the caller vouches that the kernel in front writes no length, no block table and no page but the newest tokens'; else the launch is an ordinary one.
 IL_EXPORT int il_attn_decode(const void* qkv, int row_stride, void* out, const void* cache, const int* block_table,
                              int bt_stride, const int* entry_kvlen, int page_size, int n_decode, int nh, int nkv, int hd,
                              float scale, int window, int pages_per_split, int n_splits, float* o_part, float* ml_part,
                              const void* kv_map, int* status, const float* sink, int v_is_k, const float* dist_bias, int dist_far,
-                             int sigmoid, float cap, cudaStream_t stream) {
+                             int sigmoid, float cap, int early, cudaStream_t stream) {
     if (n_decode <= 0) return IL_OK;
     if (cap > 0.f && (sigmoid || dist_bias)) return IL_BAD_ARG;
     if (sigmoid && sink) return IL_BAD_ARG;       // a sink is a term of a softmax's denominator
@@ -613,7 +616,7 @@ IL_EXPORT int il_attn_decode(const void* qkv, int row_stride, void* out, const v
     if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || pages_per_split < 0 || n_splits <= 0) return IL_BAD_ARG;
     if (n_splits > AD_MAX_SPLITS) return IL_UNSUPPORTED;
     return ad_launch(qkv, row_stride, out, cache, block_table, bt_stride, entry_kvlen, n_decode, nh, nkv, scale, window,
-                     pages_per_split, n_splits, o_part, ml_part, stream, (const CUtensorMap*)kv_map, status, sink, v_is_k, dist_bias, dist_far, sigmoid, cap);
+                     pages_per_split, n_splits, o_part, ml_part, stream, (const CUtensorMap*)kv_map, status, sink, v_is_k, dist_bias, dist_far, sigmoid, cap, early);
 }
 
 // Writes four tensor maps (4 x 128 bytes at `out_maps`) of one layer's cache, [pages][2][kv heads][16][head_dim] bfloat16:

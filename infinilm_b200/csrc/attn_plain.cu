@@ -70,8 +70,10 @@ __device__ __forceinline__ void at_store(TA* orow, int hd, int lane, const float
     }
 }
 
+// (Here and in the next kernel q, the cache and the block table may come from the kernel in front - of pages read back from 8-bit codes all of them do -: not declared __restrict__, so
+// that no load of them is moved above the wait.)
 template <typename TA, int HDP, bool SIG, bool CAP, int R>
-__global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 2 : 4) attn_tile_kernel(const TA* qkv, int row_stride, TA* __restrict__ out, const TA* cache, const int* __restrict__ block_table,
+__global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 2 : 4) attn_tile_kernel(const TA* qkv, int row_stride, TA* __restrict__ out, const TA* cache, const int* block_table,
                                  int bt_stride, const int* __restrict__ tok_pos, const int* __restrict__ tok_entry, int page_size, int page_shift,
                                  int nh, int nkv, int hd, float scale, int window, const float* __restrict__ sink,
                                  const float* __restrict__ dist_bias, int dist_far, float cap, int HW, int KS, int async) {
@@ -258,7 +260,7 @@ __device__ __forceinline__ il_f2 at_load2(const __nv_bfloat16* p, int left, bool
 
 template <typename TA, int HDP, bool SIG, bool CAP, int V>
 __global__ void __launch_bounds__(AT_DIRECT_WARPS * 32) attn_direct_kernel(const TA* qkv, int row_stride, TA* __restrict__ out, const TA* cache,
-                                                                          const int* __restrict__ block_table, int bt_stride, const int* __restrict__ tok_pos,
+                                                                          const int* block_table, int bt_stride, const int* __restrict__ tok_pos,
                                                                           const int* __restrict__ tok_entry, int page_size, int page_shift, int nh, int nkv, int hd,
                                                                           float scale, int window, const float* __restrict__ sink,
                                                                           const float* __restrict__ dist_bias, int dist_far, float cap, int vec) {

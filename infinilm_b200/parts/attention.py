@@ -85,7 +85,7 @@ class PagedAttend:
         return max(1, min(target // base, (max_pages + 3) // 4, 128))
 
     def run_quant(self, qkv, out, ctx, cache) -> None:
-        """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and `run` attends over those."""
+        """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and attended over as a plain cache's."""
         n_dec, E, width = ctx.n_decode, ctx.n_entries, cache.block_table.shape[1]
         fast = (self.dtype == torch.bfloat16 and not self.force_plain and self.hd in ops.QUANT_HEAD_DIMS and self.sink is None and self.dist_bias is None
                 and not self.sigmoid and self.cap is None)
@@ -103,12 +103,19 @@ class PagedAttend:
         pages, tma_map = ops.unpacked_cache(ctx.ws, ops.unpacked_room(cache.storage, E, width), self.nkv, self.hd, self.dtype)
         table = ctx.ws.flat("kv_unpacked_table", E * width, torch.int32).view(E, width)
         ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, nan_in_keys=True, packed=True)
-        self.run(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None))
+        # (pages and table come from the kernel in front of the attention, which therefore must not read them early)
+        self.run_pages(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None), cached_before=False)
 
     def run(self, qkv, out, ctx, cache) -> None:
         if getattr(cache, "quant", None) is not None:
-            return self.run_quant(qkv, out, ctx, cache)
+            self.run_quant(qkv, out, ctx, cache)
+        else:
+            self.run_pages(qkv, out, ctx, cache)
+
+    def run_pages(self, qkv, out, ctx, cache, cached_before: bool = True) -> None:
+        """Over pages of keys and values. cached_before: lengths, block table and all pages but the newest tokens' are older than the kernel in front."""
         G = self.nh // self.nkv
+        n_dec, E = ctx.n_decode, ctx.n_entries
         if not self.fast_ok(cache.page_size):
             if self.dtype == torch.bfloat16 and not self.force_plain and not PagedAttend._warned_plain:
                 PagedAttend._warned_plain = True
@@ -120,7 +127,6 @@ class PagedAttend:
                                 cache.page_size, self.nh, self.nkv, self.hd, self.scale, self.mask_arg, self.sink, self.dist_bias, self.sigmoid,
                                 self.cap)
             return
-        n_dec, E = ctx.n_decode, ctx.n_entries
         if n_dec > 0:
             max_len = max(ctx.h_kvlen[:n_dec])
             if self.span is not None:
@@ -134,7 +140,7 @@ class PagedAttend:
                                  self.nh, self.nkv, self.hd, self.scale, self.mask_arg, 0, n_splits,
                                  ctx.ws.flat("attn_o_part", rows * self.hd, torch.float32),
                                  ctx.ws.flat("attn_ml_part", rows * 2, torch.float32), kv_map=cache.tma_map, sink=self.sink,
-                                 v_is_k=v_is_k, dist_bias=self.dist_bias, sigmoid=self.sigmoid, cap=self.cap)
+                                 v_is_k=v_is_k, dist_bias=self.dist_bias, sigmoid=self.sigmoid, cap=self.cap, cached_before=cached_before)
         if E > n_dec:
             # prompt portions: on tcgen05 with tensor memory where the head size has that kernel (64, 128, 256) and the cache
             # its tensor map; else the mma.sync kernel. The tile is 128 (64) rows = tokens x heads of a kv head.

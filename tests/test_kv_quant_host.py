@@ -1,0 +1,76 @@
+"""What the host does around the 8-bit cache's kernels (no GPU): which kernels a step takes and what it vouches for."""
+import inspect
+import os
+import re
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from infinilm_b200 import ops
+from infinilm_b200.cache import PagedKVView
+from infinilm_b200.engine.step import Workspace
+from infinilm_b200.parts.attention import PagedAttend
+
+LAUNCHING = ("attention_decode_quant", "attention_prefill_quant", "kv_unpack", "attention_decode", "attention_plain", "attention_prefill", "attention_prefill_tc5")
+SIGNATURES = {name: inspect.signature(getattr(ops, name)) for name in LAUNCHING}
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "infinilm_b200", "csrc")
+
+
+def _source(name):
+    with open(os.path.join(CSRC, name), encoding="utf-8") as fh:
+        return re.sub(r"//[^\n]*", "", fh.read())
+
+
+def _step(monkeypatch, nh, nkv, hd, dtype=torch.bfloat16, n_dec=2, portions=(), quant="int8", prefill="auto"):
+    """The kernels that an attention's step launches, as (name, arguments): n_dec requests of one token, then portions."""
+    calls = []
+    for name in LAUNCHING:
+        def record(*a, _name=name, **kw):
+            bound = SIGNATURES[_name].bind(*a, **kw)
+            bound.apply_defaults()
+            calls.append((_name, bound.arguments))
+        monkeypatch.setattr(ops, name, record)
+    monkeypatch.setattr(ops, "kv_tensor_map", lambda t: None)
+    monkeypatch.setattr(ops, "attention_decode_resident_blocks", lambda *a: 296)
+    E, T, pages, width = n_dec + len(portions), n_dec + sum(portions), 12, 3
+    kvlen = [40] * n_dec + [max(p, 30) for p in portions]
+    ctx = SimpleNamespace(n_decode=n_dec, n_entries=E, ws=Workspace("cpu", 64), h_kvlen=kvlen, entry_kvlen=torch.tensor(kvlen, dtype=torch.int32),
+                          entry_qstart=torch.zeros(E + 1, dtype=torch.int32), tok_pos=torch.arange(T, dtype=torch.int32), tok_entry=torch.arange(T, dtype=torch.int32),
+                          prompt_tiles=lambda n: max(1, len(portions)))
+    storage = torch.zeros((pages, nkv, ops.kv_quant_record(hd)), dtype=torch.uint8) if quant else torch.zeros((pages, 2, nkv, 16, hd), dtype=dtype)
+    view = PagedKVView(storage, torch.zeros((E, width), dtype=torch.int32), 16, max_pages=width, quant=quant)
+    core = PagedAttend(dtype, nh, nkv, hd, 0.1, prefill_kernel=prefill)
+    core.run(torch.zeros((T, nh * hd), dtype=dtype), torch.zeros((T, nh * hd), dtype=dtype), ctx, view)
+    return calls
+
+
+# ---- what is read before a kernel's wait ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd", [16, 32, 48, 80, 96, 112, 192])
+def test_pages_read_back_are_not_read_early(monkeypatch, hd):
+    """The decode kernel reads the block table and pages before its wait only where its caller says that the kernel in front wrote neither; kv_unpack in front writes both."""
+    assert SIGNATURES["attention_decode"].parameters["cached_before"].default is False
+    calls = _step(monkeypatch, 4, 2, hd)
+    assert [c[0] for c in calls] == ["kv_unpack", "attention_decode"]
+    assert calls[1][1]["block_table"].data_ptr() == calls[0][1]["table"].data_ptr() and calls[1][1]["cached_before"] is False
+    calls = _step(monkeypatch, 4, 2, hd, quant=None)
+    assert [c[0] for c in calls] == ["attention_decode"] and calls[0][1]["cached_before"] is True
+    calls = _step(monkeypatch, 4, 2, 64)
+    assert [c[0] for c in calls] == ["attention_decode_quant"] and calls[0][1]["cached_before"] is True
+
+
+def test_the_decode_kernel_starts_early_only_where_it_may():
+    text = _source("attn_decode.cu")
+    launches = re.findall(r"(\w+)\(\s*\(?([^;]{0,40}?)attn_decode_kernel<", text)
+    assert [(f, a.strip()) for f, a in launches if f.startswith("il_launch") or f == "IL_LAUNCH"] == [("il_launch_as", "early != 0,")]
+
+
+def test_the_plain_kernels_do_not_declare_the_block_table_read_only():
+    """They wait first, and the kernel in front may have written the table (kv_unpack does)."""
+    found = 0
+    for kernel in re.split(r"__global__", _source("attn_plain.cu"))[1:]:
+        head, body = kernel.split("{", 1)
+        if re.search(r"il_pdl_(?:wait|begin)\(", body):
+            found += 1
+            assert re.search(r"const int\s*\* block_table", head), head
+    assert found == 2
