@@ -85,7 +85,8 @@ class PagedAttend:
         return max(1, min(target // base, (max_pages + 3) // 4, 128))
 
     def run_quant(self, qkv, out, ctx, cache) -> None:
-        """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and attended over as a plain cache's."""
+        """The same over a cache of 8-bit codes: its own kernels where the compute dtype and the head size have them, else the pages are read back and attended over as a plain cache's
+        (for the rows that no kernel over codes has been through)."""
         n_dec, E, width = ctx.n_decode, ctx.n_entries, cache.block_table.shape[1]
         fast = (self.dtype == torch.bfloat16 and not self.force_plain and self.hd in ops.QUANT_HEAD_DIMS and self.sink is None and self.dist_bias is None
                 and not self.sigmoid and self.cap is None)
@@ -100,11 +101,12 @@ class PagedAttend:
                                         self.nh, self.nkv, self.hd, self.scale, self.mask_arg, ctx.ws, n_tiles_rule=(qkv.shape[0] - n_dec + per - 1) // per + E - n_dec - 1,
                                         room=ops.unpacked_room(cache.storage, E - n_dec, width))
             return
-        pages, tma_map = ops.unpacked_cache(ctx.ws, ops.unpacked_room(cache.storage, E, width), self.nkv, self.hd, self.dtype)
+        first = n_dec if fast else 0
+        pages, tma_map = ops.unpacked_cache(ctx.ws, ops.unpacked_room(cache.storage, E - first, width), self.nkv, self.hd, self.dtype)
         table = ctx.ws.flat("kv_unpacked_table", E * width, torch.int32).view(E, width)
-        ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, nan_in_keys=True, packed=True)
+        ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, first_entry=first, nan_in_keys=True, packed=True)
         # (pages and table come from the kernel in front of the attention, which therefore must not read them early)
-        self.run_pages(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None), cached_before=False)
+        self.run_pages(qkv, out, ctx, dataclasses.replace(cache, storage=pages, block_table=table, tma_map=tma_map, quant=None), first, cached_before=False)
 
     def run(self, qkv, out, ctx, cache) -> None:
         if getattr(cache, "quant", None) is not None:
@@ -112,8 +114,9 @@ class PagedAttend:
         else:
             self.run_pages(qkv, out, ctx, cache)
 
-    def run_pages(self, qkv, out, ctx, cache, cached_before: bool = True) -> None:
-        """Over pages of keys and values. cached_before: lengths, block table and all pages but the newest tokens' are older than the kernel in front."""
+    def run_pages(self, qkv, out, ctx, cache, first: int = 0, cached_before: bool = True) -> None:
+        """Over pages of keys and values, for the entries from `first` on (0 or the step's n_decode). cached_before: lengths, block table and all pages but the newest tokens' are
+        older than the kernel in front."""
         G = self.nh // self.nkv
         n_dec, E = ctx.n_decode, ctx.n_entries
         if not self.fast_ok(cache.page_size):
@@ -123,11 +126,15 @@ class PagedAttend:
                               f"the fast bfloat16 kernels (pages of 16 or a multiple, at most {self.FAST_MAX_GROUP} heads per kv head, "
                               "head sizes in steps of 16 up to 256): the plain kernel runs, at a fraction of their speed",
                               RuntimeWarning, stacklevel=2)
-            ops.attention_plain(qkv, out, cache.storage, cache.block_table, ctx.tok_pos, ctx.tok_entry,
+            if first:                             # (an entry of the first n_decode is one row)
+                qkv, out, tok_pos, tok_entry = qkv[first:], out[first:], ctx.tok_pos[first:], ctx.tok_entry[first:]
+            else:
+                tok_pos, tok_entry = ctx.tok_pos, ctx.tok_entry
+            ops.attention_plain(qkv, out, cache.storage, cache.block_table, tok_pos, tok_entry,
                                 cache.page_size, self.nh, self.nkv, self.hd, self.scale, self.mask_arg, self.sink, self.dist_bias, self.sigmoid,
                                 self.cap)
             return
-        if n_dec > 0:
+        if n_dec > first:
             max_len = max(ctx.h_kvlen[:n_dec])
             if self.span is not None:
                 max_len = min(max_len, self.span + self.FAST_PAGE)

@@ -74,3 +74,25 @@ def test_the_plain_kernels_do_not_declare_the_block_table_read_only():
             found += 1
             assert re.search(r"const int\s*\* block_table", head), head
     assert found == 2
+
+
+# ---- a step's rows are attended to once --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nh,nkv,prefill,behind", [(4, 2, "mma", "attention_prefill"), (132, 1, "auto", "attention_plain"), (70, 1, "mma", "attention_plain")])
+def test_single_tokens_beside_portions_are_attended_to_once(monkeypatch, nh, nkv, prefill, behind):
+    """Where portions have no kernel over codes, only their pages are read back, and only their rows go through the kernels over pages."""
+    calls = _step(monkeypatch, nh, nkv, 64, n_dec=2, portions=(5, 9), prefill=prefill)
+    assert [c[0] for c in calls] == ["attention_decode_quant", "kv_unpack", behind]
+    unpack, last = calls[1][1], calls[2][1]
+    assert unpack["first_entry"] == 2
+    if behind == "attention_plain":
+        assert last["qkv"].shape[0] == last["out"].shape[0] == 14 and last["tok_pos"].tolist() == last["tok_entry"].tolist() == list(range(2, 16))
+        assert last["qkv"].is_contiguous() and last["out"].is_contiguous()
+    else:
+        assert (last["first_entry"], last["n_entries"]) == (2, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_head_sizes_without_kernels_over_codes_read_all_entries_back(monkeypatch, dtype):
+    calls = _step(monkeypatch, 4, 2, 48, dtype=dtype, portions=(5,))
+    assert calls[0][0] == "kv_unpack" and calls[0][1]["first_entry"] == 0
+    assert [c[0] for c in calls[1:]] == (["attention_plain"] if dtype is torch.float32 else ["attention_decode", "attention_prefill"])

@@ -1,0 +1,53 @@
+"""Steps over the 8-bit cache that mix single tokens and prompt portions, by every path that such a step can take, against attention in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import plain_kv_quant as P
+from test_parts_gpu import _ctx
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kind", ["fp8_e4m3", "int8"])
+@pytest.mark.parametrize("nh,nkv,hd,prefill", [(4, 2, 64, "mma"), (4, 2, 128, "mma"), (2, 1, 256, "mma"), (4, 2, 128, "auto"), (132, 1, 64, "auto"), (70, 1, 64, "mma"), (4, 2, 96, "auto")])
+@pytest.mark.parametrize("window", [None, 24])
+def test_single_tokens_beside_portions(cuda_device, kind, nh, nkv, hd, prefill, window):
+    """Two requests with a token each, then portions of 5 and 40 tokens: every row is right, and the single tokens' bits are those of a step without portions."""
+    from infinilm_b200 import ops
+    from infinilm_b200.cache import PagedKVView
+    from infinilm_b200.parts.attention import PagedAttend
+    starts, qlens = [60, 29, 33, 10], [1, 1, 5, 40]
+    kvlens = [s + n for s, n in zip(starts, qlens)]
+    need = [(n + 15) // 16 for n in kvlens]
+    g = torch.Generator().manual_seed(41)
+    ids, rows, at = torch.randperm(sum(need) + 2, generator=g).tolist(), [], 0
+    for n in need:
+        rows.append(ids[at:at + n] + [-1] * (max(need) - n))
+        at += n
+    rec = P.make_records(torch.randn((sum(need) + 2, nkv, 2, 16, hd), generator=g), kind)
+    val = P.decode_records(rec, hd, kind)
+    q = torch.randn((sum(qlens), nh * hd), generator=g).to(torch.bfloat16)
+    core = PagedAttend(torch.bfloat16, nh, nkv, hd, 1.0 / math.sqrt(hd), window, prefill_kernel=prefill)
+
+    def go(entries):
+        ctx = _ctx("bfloat16", starts[:entries], qlens[:entries])
+        out = torch.full((sum(qlens[:entries]), nh * hd), 3.0, dtype=torch.bfloat16, device="cuda")
+        core.run(q[:out.shape[0]].cuda(), out, ctx, PagedKVView(rec.cuda(), _i32(rows[:entries]), 16, True, max(need), quant=kind))
+        return out.cpu()
+    got = go(4)
+    if hd in ops.QUANT_HEAD_DIMS:
+        assert torch.equal(got[:2], go(2))
+    t = 0
+    for e in range(4):
+        for i in range(qlens[e]):
+            want, mag = P.attend(q[t].view(nh, hd), val, rows[e], starts[e] + i, 1.0 / math.sqrt(hd), window or 0)
+            # one rounding of the output, one of each weight (bfloat16 at most: 2^-8, and its sum's), sums in 32 bits
+            assert ((got[t].double().view(nh, hd) - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -7) * want.abs() + (2.0 ** -8 + 2.0 ** -14) * mag).all(), (e, i)
+            t += 1
+    ops.check_status("cuda:0")
