@@ -8,7 +8,8 @@
 // product. The exponent of K multiplies the score; the exponent of V joins the softmax's: with t_k = s_k log2 e + f_k and the running
 // maximum taken over t_k, the weight w_k = 2^(t_k - m) is what V's codes are multiplied by, at most 2^8 and therefore a half with 11 bits
 // where they count, and the denominator adds w_k 2^-f_k in 32 bits. One exponential a score, as without a quantised cache. q goes to halves times a
-// power of two of its row's (its largest magnitude then lies in 2^14 .. 2^15): what a half cannot hold of it is below 2^-39 of that.
+// power of two of its row's (its largest magnitude then lies in 2^8 .. 2^9, so that a score times the largest power of two of K, 2^100, stays within 32 bits): what a half
+// cannot hold of it is below 2^-33 of that.
 //
 //   Products: S^T = K.Q^T and O^T = V^T.P^T, keys and V's columns as the 16 rows of a tile, heads as its 8 columns (NT tiles: one up to eight heads a kv head, two
 //   beyond): with the heads as rows, half of every product, softmax and register would belong to rows that are not there where a kv head has eight heads or fewer.
@@ -283,8 +284,8 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
 #pragma unroll
             for (int k = 1; k < DQ_CH; k <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, k));
             const int ex = max((int)(most >> 7) - 127, -100);
-            const float up = __int_as_float((127 + 14 - ex) << 23);
-            if (c == 0) q_scale[r] = scale_log2 * __int_as_float((127 - 14 + ex) << 23);
+            const float up = __int_as_float((127 + 8 - ex) << 23);
+            if (c == 0) q_scale[r] = scale_log2 * __int_as_float((127 - 8 + ex) << 23);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * k]), b = *reinterpret_cast<const __nv_bfloat162*>(&x[2 * k + 1]);

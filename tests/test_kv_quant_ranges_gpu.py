@@ -1,0 +1,60 @@
+"""Single tokens over the 8-bit cache where values differ most: keys and queries whose powers of two are far apart. Against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import plain_kv_quant as P
+
+pytestmark = pytest.mark.gpu
+KINDS = ["fp8_e4m3", "int8"]
+HEADS = [(4, 1, 64), (12, 1, 64), (8, 1, 128), (16, 1, 128), (4, 1, 256), (16, 1, 256)]      # one and two column tiles of heads
+
+
+def _run(dev, monkeypatch, q, kv, kind, blocks, scale, order=None, window=None):
+    """One request over kv [keys, kv_heads, 2, head_dim] (pages in `order`); its output, the 64-bit one, and the sums of weight times |value|."""
+    from infinilm_b200 import ops
+    from infinilm_b200.engine.step import Workspace
+    n, nkv, _, hd = kv.shape
+    nh, pages = q.shape[0], (n + 15) // 16
+    full = torch.cat([kv.double(), torch.zeros((pages * 16 - n, nkv, 2, hd), dtype=torch.float64)]).view(pages, 16, nkv, 2, hd).permute(0, 2, 3, 1, 4).contiguous()
+    rec = P.make_records(full, kind)
+    val = P.decode_records(rec, hd, kind)
+    ids = torch.randperm(pages, generator=torch.Generator().manual_seed(5))
+    placed = torch.empty_like(rec)
+    placed[ids] = rec
+    monkeypatch.setattr(ops, "_quant_blocks", lambda *a: blocks)
+    out = torch.full((1, nh * hd), 3.0, dtype=torch.bfloat16, device=dev)
+    ops.attention_decode_quant(q.reshape(1, -1).to(dev), out, placed.to(dev), kind, ids.to(torch.int32).view(1, -1).to(dev), torch.tensor([n], dtype=torch.int32, device=dev), 1, nh,
+                               nkv, hd, scale, window, n, Workspace(dev, 16))
+    ops.check_status(dev)
+    rows = val.permute(0, 3, 1, 2, 4).reshape(pages * 16, nkv, 2, hd)[:n]
+    want, mag = [], []
+    for h in range(nh):
+        k, v = rows[:, h // (nh // nkv), 0], rows[:, h // (nh // nkv), 1]
+        p = torch.softmax(k @ q[h].double() * scale, 0)
+        want.append(p @ v), mag.append(p @ v.abs())
+    return out.cpu().double().view(nh, hd), torch.stack(want), torch.stack(mag)
+
+
+def _check(got, want, mag, n):
+    # the output's rounding; weights as halves, 2^-11 each (below 2^-14 of the largest: 2^-25 of it a key, its row's largest code half of the largest there is); exponentials, exponents and
+    # sums in 32 bits: 2^-15 together
+    room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -24 * n * mag.amax(-1, keepdim=True)
+    off = (got - want).abs()
+    assert (off <= room).all(), float((off / room.clamp(min=1e-300)).max())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("up", [1, -1])
+def test_large_keys_with_small_queries(cuda_device, monkeypatch, kind, nh, nkv, hd, up):
+    """Scores of ordinary size from keys near 2^106 and queries near 2^-98, and the other way round."""
+    g = torch.Generator().manual_seed(35)
+    n, sign = 150, torch.sign(torch.randn(hd, generator=g)).double()
+    kv = torch.randn((n, nkv, 2, hd), generator=g).double()
+    k_size, q_size = (2.0 ** 106, 2.0 ** -98) if up > 0 else (2.0 ** -85, 2.0 ** 93)
+    kv[:, :, 0] = k_size * sign * (1 + 0.2 * torch.rand((n, nkv, hd), generator=g).double()) * (0.5 + 0.5 * torch.rand((n, 1, 1), generator=g).double())
+    q = (q_size * sign * (1 + 0.1 * torch.rand((nh, hd), generator=g).double())).to(torch.bfloat16)
+    got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, 0, 8.0 / (hd * 2.0 ** 8))
+    _check(got, want, mag, n)
