@@ -7,7 +7,8 @@
 // Codes become halves (exactly) in registers and go straight into m16n8k16 products with f32 sums; nothing is scaled before a
 // product. The exponent of K multiplies the score; the exponent of V joins the softmax's: with t_k = s_k log2 e + f_k and the running
 // maximum taken over t_k, the weight w_k = 2^(t_k - m) is what V's codes are multiplied by, at most 2^8 and therefore a half with 11 bits
-// where they count, and the denominator adds w_k 2^-f_k in 32 bits. One exponential a score, as without a quantised cache. q goes to halves times a
+// where they count, and the denominator adds w_k 2^-f_k in 32 bits (2^-100 to 2^108 a key). Where exponents of V lie so far apart
+// that w_k may be 0 although p_k counts, the denominator's 2^(t_k - f_k - m) is an exponential of its own. Else one a score, as without a quantised cache. q goes to halves times a
 // power of two of its row's (its largest magnitude then lies in 2^8 .. 2^9, so that a score times the largest power of two of K, 2^100, stays within 32 bits): what a half
 // cannot hold of it is below 2^-33 of that.
 //
@@ -62,6 +63,9 @@ __host__ __device__ constexpr int dq_smem(int rows) { return dq_q(rows) + rows *
 constexpr int dq_per_sm(int kind, int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 2 && kind == KVQ_INT8 ? 3 : 4) : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
 constexpr float DQ_RAISE = 8.f;                   // the running maximum follows only when a page's is more than this above it (log2 units)
+// Bytes of V's exponents that are in order: 2^-80 .. 2^-1 (rows up to 224 in e4m3, 63 as whole numbers). Among these a weight that is flushed to 0, below 2^-126, has a score 2^46 below the best
+// one: no share of the denominator.
+constexpr unsigned DQ_V_LOW = 47, DQ_V_SPAN = 80;
 
 __device__ __forceinline__ void dq_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -99,6 +103,13 @@ __device__ __forceinline__ float dq_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float dq_ex2_small(float x) {              // ... down to 2^-149
+    const float root = dq_ex2(0.5f * x);
+    return root * root;
+}
+// The root of the factor that brings sums from the reference m to M >= m (m = -infinity: there are none). A denominator may be near 2^108 where the factor is below 2^-126: it is
+// multiplied by the root twice.
+__device__ __forceinline__ float dq_root(float m, float M) { return m == -INFINITY ? 0.f : dq_ex2(0.5f * (m - M)); }
 __device__ __forceinline__ uint32_t dq_pack_half(float lo, float hi) {
     uint32_t h;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(hi), "f"(lo));
@@ -311,6 +322,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
         il_f2 l[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -FLT_MAX, l[j] = il_f2_dup(0.f);
+        unsigned v_low = DQ_V_LOW;
         for (int it = 0; it < n_my; ++it) {
             if (!dq_wait(bars + (done + it) % DQ_STAGES * 8, (done + it) / DQ_STAGES & 1)) {
                 if (lane == 0) atomicExch(status, 91);
@@ -358,11 +370,12 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
             const int page0 = (p0 + warp + it * DQ_WARPS) * KVQ_PAGE;
             const bool gone = (bad >> (it & 31)) & 1, edge = gone || page0 < lo || page0 + KVQ_PAGE > kvlen;
             float tv[NT][4], inv_v[2];
+            bool odd[2];                          // an exponent of V out of order
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const uint32_t ke = rec[2 * KVQ_PAGE * DQ_HD + 8 * n + lg], ve = rec[2 * KVQ_PAGE * DQ_HD + KVQ_PAGE + 8 * n + lg];
                 const float kp = __uint_as_float(ke << 23 | 1u), add = __uint_as_float(0x4b000000u | ve) - 8388735.f;     // (2^23 + byte as a float has the byte in its lowest bits)
-                inv_v[n] = __uint_as_float(0x7f000001u - (ve << 23));
+                inv_v[n] = __uint_as_float(0x7f000001u - (ve << 23)), odd[n] = ve - v_low >= DQ_V_SPAN;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
                     il_f2_get(il_f2_fma(il_f2_mul(il_f2_make(s[j][2 * n], s[j][2 * n + 1]), il_f2_dup(kp)), s_scale[j], il_f2_dup(add)), tv[j][2 * n], tv[j][2 * n + 1]);
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
                 for (int n = 0; n < 2; ++n) {
                     const int key = page0 + 8 * n + lg;
                     if (gone || key < lo || key >= kvlen) {
-                        inv_v[n] = 0.f;
+                        inv_v[n] = 0.f, odd[n] = false;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) tv[j][2 * n] = tv[j][2 * n + 1] = -INFINITY;
                     }
@@ -395,22 +408,37 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
                     top = fmaxf(fmaxf(top, dv[j][2 * n]), dv[j][2 * n + 1]);
                 }
             }
-            if (__any_sync(0xffffffffu, top > DQ_RAISE)) {           // also the first keys of a head
+            if (__any_sync(0xffffffffu, top > DQ_RAISE || odd[0] || odd[1])) {           // also the first keys of a head
+                const bool far = __any_sync(0xffffffffu, odd[0] || odd[1]);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    float corr[2];
+                    float root[2], corr[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float mx = fmaxf(tv[j][i], tv[j][2 + i]);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                         const float mn = mx > m[j][i] + DQ_RAISE ? mx : m[j][i];
-                        corr[i] = dq_ex2(m[j][i] - mn);           // 0 when nothing was summed yet
+                        root[i] = dq_root(m[j][i], mn), corr[i] = root[i] * root[i];      // 0 when nothing was summed yet
                         m[j][i] = mn, dv[j][i] = tv[j][i] - mn, dv[j][2 + i] = tv[j][2 + i] - mn;
                     }
-                    l[j] = il_f2_mul(l[j], il_f2_make(corr[0], corr[1]));
+                    l[j] = il_f2_mul(il_f2_mul(l[j], il_f2_make(root[0], root[1])), il_f2_make(root[0], root[1]));
 #pragma unroll
                     for (int t = 0; t < DQ_MT; ++t) o[t][j][0] *= corr[0], o[t][j][1] *= corr[1], o[t][j][2] *= corr[0], o[t][j][3] *= corr[1];
+                }
+                if (__builtin_expect(far, 0)) {   // a key's share of the denominator by an exponential of its own: its weight may be flushed to 0 where its score counts all the same
+                    bool above = false;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const int v = (int)(0x7f000001u - __float_as_uint(inv_v[n]) >> 23);       // the exponent's byte again; of a masked key 254
+                        above = above || (v >= (int)(DQ_V_LOW + DQ_V_SPAN) && v <= KVQ_MOST + 127);
+                        if (v == KVQ_NAN) continue;           // (stays NaN)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            l[j] = il_f2_add(l[j], il_f2_make(dq_ex2_small(dv[j][2 * n] - (float)(v - 127)), dq_ex2_small(dv[j][2 * n + 1] - (float)(v - 127))));
+                        inv_v[n] = 0.f;
+                    }
+                    if (__any_sync(0xffffffffu, above)) v_low = 256u;     // what is in order so far may be far below this one: every page of the stretch from here on
                 }
             }
             uint32_t pf[NT][2];
@@ -509,7 +537,8 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
 #pragma unroll
             for (int w = 0; w < DQ_WARPS; ++w) {
                 const float mw = sm_ml[(w * ROWS + r) * 2];
-                L += (mw == -INFINITY ? 0.f : dq_ex2(mw - M)) * sm_ml[(w * ROWS + r) * 2 + 1];
+                const float root = dq_root(mw, M);
+                L += sm_ml[(w * ROWS + r) * 2 + 1] * root * root;
             }
             *reinterpret_cast<float2*>(sm_ml + (DQ_WARPS * ROWS + r) * 2) = make_float2(M, L);
         }
@@ -551,8 +580,8 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
 #pragma unroll
             for (int p = 0; p < DQ_CLUSTER; ++p)
                 if (p < per_unit && ml[p].x != -INFINITY) {           // (no part: what lies there is not one)
-                    const float f = dq_ex2(ml[p].x - M);
-                    L += f * ml[p].y, acc.x += f * v[p].x, acc.y += f * v[p].y, acc.z += f * v[p].z, acc.w += f * v[p].w;
+                    const float root = dq_root(ml[p].x, M), f = root * root;
+                    L += ml[p].y * root * root, acc.x += f * v[p].x, acc.y += f * v[p].y, acc.z += f * v[p].z, acc.w += f * v[p].w;
                 }
             dq_write(acc, M, L, out + ((size_t)i * nh + head0) * DQ_HD, nullptr, nullptr, r, d);
         }
@@ -607,22 +636,22 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 32 : 128) attn_decode_quant_me
         float mx = M;
 #pragma unroll
         for (int k = 0; k < DQM_ROUND; ++k) mx = fmaxf(mx, ml[k].x);
-        const float corr = M == -INFINITY ? 0.f : dq_ex2(M - mx);
-        M = mx, L *= corr;
+        const float back = dq_root(M, mx), corr = back * back;
+        M = mx, L = L * back * back;
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[c][0] *= corr, acc[c][1] *= corr, acc[c][2] *= corr, acc[c][3] *= corr;
 #pragma unroll
         for (int k = 0; k < DQM_ROUND; ++k) {
-            const float f = ml[k].x == -INFINITY ? 0.f : dq_ex2(ml[k].x - M);
-            L += f * ml[k].y;                     // (a NaN of a part that is there stays one)
+            const float root = dq_root(ml[k].x, M), f = root * root;
+            L += ml[k].y * root * root;           // (a NaN of a part that is there stays one)
 #pragma unroll
             for (int c = 0; c < NC; ++c) acc[c][0] += f * v[c][k].x, acc[c][1] += f * v[c][k].y, acc[c][2] += f * v[c][k].z, acc[c][3] += f * v[c][k].w;
         }
     }
 #pragma unroll
     for (int x = LPR; x < 32; x <<= 1) {          // lanes that had other parts of the same columns
-        const float Mo = __shfl_xor_sync(0xffffffffu, M, x), mx = fmaxf(M, Mo), f = M == -INFINITY ? 0.f : dq_ex2(M - mx);
-        L *= f, L += __shfl_xor_sync(0xffffffffu, L, x);
+        const float Mo = __shfl_xor_sync(0xffffffffu, M, x), mx = fmaxf(M, Mo), root = dq_root(M, mx), f = root * root;
+        L = L * root * root, L += __shfl_xor_sync(0xffffffffu, L, x);
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[0][c] *= f, acc[0][c] += __shfl_xor_sync(0xffffffffu, acc[0][c], x);
         M = mx;
@@ -639,7 +668,10 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 32 : 128) attn_decode_quant_me
 #pragma unroll
         for (int w = 0; w < WPR; ++w) M = fmaxf(M, sums[w].x);
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) f[w] = sums[w].x == -INFINITY ? 0.f : dq_ex2(sums[w].x - M), L += f[w] * sums[w].y;
+        for (int w = 0; w < WPR; ++w) {
+            const float root = dq_root(sums[w].x, M);
+            f[w] = root * root, L += sums[w].y * root * root;
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;

@@ -1,4 +1,4 @@
-"""Single tokens over the 8-bit cache where values differ most: keys and queries whose powers of two are far apart. Against 64 bits."""
+"""Single tokens over the 8-bit cache where values differ most: exponents as far apart as the format lets them be, keys and queries whose powers of two are far apart. Against 64 bits."""
 import math
 
 import pytest
@@ -9,6 +9,7 @@ import plain_kv_quant as P
 pytestmark = pytest.mark.gpu
 KINDS = ["fp8_e4m3", "int8"]
 HEADS = [(4, 1, 64), (12, 1, 64), (8, 1, 128), (16, 1, 128), (4, 1, 256), (16, 1, 256)]      # one and two column tiles of heads
+BLOCKS = [0, 1, 3, 300, -2, -8]
 
 
 def _run(dev, monkeypatch, q, kv, kind, blocks, scale, order=None, window=None):
@@ -43,6 +44,29 @@ def _check(got, want, mag, n):
     room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -24 * n * mag.amax(-1, keepdim=True)
     off = (got - want).abs()
     assert (off <= room).all(), float((off / room.clamp(min=1e-300)).max())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", BLOCKS)
+@pytest.mark.parametrize("how", ["pair", "rising", "falling", "mixed"])
+def test_values_whose_exponents_lie_as_far_apart_as_they_can(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, how):
+    """The sum of weights counts every key, however small its value beside another's: in one page, page after page of a warp, warp beside warp, block beside block."""
+    g = torch.Generator().manual_seed(33)
+    n = 400
+    kv = torch.randn((n, nkv, 2, hd), generator=g).double()
+    if how == "pair":
+        e = torch.full((n,), -60.0)
+        e[211] = 70.0
+    elif how in ("rising", "falling"):
+        e = torch.linspace(-90, 98, n).round()
+        e = e if how == "rising" else e.flip(0)
+    else:
+        e = torch.randint(-95, 99, (n,), generator=g).float()
+    kv[:, :, 1] *= torch.exp2(e.double())[:, None, None]
+    q = torch.randn((nh, hd), generator=g).to(torch.bfloat16)
+    got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, blocks, 1.0 / math.sqrt(hd))
+    _check(got, want, mag, n)
 
 
 @pytest.mark.parametrize("kind", KINDS)
