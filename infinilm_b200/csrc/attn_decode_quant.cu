@@ -8,7 +8,7 @@
 // product. The exponent of K multiplies the score; the exponent of V joins the softmax's: with t_k = s_k log2 e + f_k and the running
 // maximum taken over t_k, the weight w_k = 2^(t_k - m) is what V's codes are multiplied by, at most 2^8 and therefore a half with 11 bits
 // where they count, and the denominator adds w_k 2^-f_k in 32 bits (2^-100 to 2^108 a key). Where exponents of V lie so far apart
-// that w_k may be 0 although p_k counts, the denominator's 2^(t_k - f_k - m) is an exponential of its own. Else one a score, as without a quantised cache. q goes to halves times a
+// that w_k may be 0 although p_k counts, the denominator's 2^(t_k - f_k - m) is an exponential of its own. A row of zeros counts as one of the lowest exponent. Else one a score, as without a quantised cache. q goes to halves times a
 // power of two of its row's (its largest magnitude then lies in 2^8 .. 2^9, so that a score times the largest power of two of K, 2^100, stays within 32 bits): what a half
 // cannot hold of it is below 2^-33 of that.
 //
@@ -410,6 +410,25 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
             }
             if (__any_sync(0xffffffffu, top > DQ_RAISE || odd[0] || odd[1])) {           // also the first keys of a head
                 const bool far = __any_sync(0xffffffffu, odd[0] || odd[1]);
+                if (__builtin_expect(far, 0)) {
+                    // A row of zeros has the exponent 2^0, far above its neighbours', and must not set the reference that their weights are rounded against: it gets the lowest.
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const int key = 8 * n + lg;
+                        uint32_t some = inv_v[n] != __uint_as_float(0x7f000001u - (127u << 23));
+                        if (!some)
+                            for (int c = lq; c < DQ_CH; c += 4) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(rec + KVQ_PAGE * DQ_HD + ((key * DQ_CH + c) ^ kvq_turn(DQ_HD, true, key)) * 16);
+                                some |= (w.x | w.y | w.z | w.w) & 0x7f7f7f7fu;        // (zeros of either sign)
+                            }
+                        some |= __shfl_xor_sync(0xffffffffu, some, 1);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 2);
+                        if (some) continue;
+                        inv_v[n] = __uint_as_float(0x7f000001u - ((unsigned)(KVQ_LEAST + 127) << 23));
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) tv[j][2 * n] += (float)KVQ_LEAST, tv[j][2 * n + 1] += (float)KVQ_LEAST;
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float root[2], corr[2];

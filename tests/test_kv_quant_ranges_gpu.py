@@ -1,4 +1,4 @@
-"""Single tokens over the 8-bit cache where values differ most: exponents as far apart as the format lets them be, keys and queries whose powers of two are far apart. Against 64 bits."""
+"""Single tokens over the 8-bit cache where values differ most: rows of zeros with the highest scores, exponents as far apart as the format lets them be, keys and queries whose powers of two are far apart. Against 64 bits."""
 import math
 
 import pytest
@@ -46,10 +46,42 @@ def _check(got, want, mag, n):
     assert (off <= room).all(), float((off / room.clamp(min=1e-300)).max())
 
 
+def _toward(hd, g):
+    u = torch.randn(hd, generator=g).double()
+    return u / u.norm()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nh,nkv,hd", HEADS)
 @pytest.mark.parametrize("blocks", BLOCKS)
-@pytest.mark.parametrize("how", ["pair", "rising", "falling", "mixed"])
+@pytest.mark.parametrize("gap,size", [(10.0, 1.0), (8.0, 2.0 ** -4), (12.0, 2.0 ** -4), (0.0, 2.0 ** -14), (14.0, 2.0 ** -14)])
+def test_a_row_of_zeros_takes_its_share_and_nothing_else(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, gap, size):
+    """Values of zero at keys whose scores lie `gap` above the others': the sum of weights is theirs, what the others bring keeps its bits. Zeros of both signs."""
+    g = torch.Generator().manual_seed(31)
+    n, u = 500, _toward(hd, g)
+    kv = 0.3 * torch.randn((n, nkv, 2, hd), generator=g).double()
+    kv[:, :, 1] *= size / 0.3
+    q = (math.sqrt(hd) * u + 0.1 * torch.randn((nh, hd), generator=g).double()).to(torch.bfloat16)
+    for at, zero in ((37, 0.0), (290, -0.0)):
+        kv[at, :, 0] = (gap * u)                  # q.K / sqrt(hd) is near `gap`
+        kv[at, :, 1] = zero
+    got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, blocks, 1.0 / math.sqrt(hd))
+    _check(got, want, mag, n)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_zeros_alone_give_zeros(cuda_device, monkeypatch, kind):
+    g = torch.Generator().manual_seed(32)
+    kv = torch.randn((70, 1, 2, 128), generator=g).double()
+    kv[:, :, 1] = 0.0
+    got, _, _ = _run(cuda_device, monkeypatch, torch.randn((8, 128), generator=g).to(torch.bfloat16), kv, kind, 0, 0.1)
+    assert not got.any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", BLOCKS)
+@pytest.mark.parametrize("how", ["pair", "rising", "falling", "mixed", "zeros"])
 def test_values_whose_exponents_lie_as_far_apart_as_they_can(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks, how):
     """The sum of weights counts every key, however small its value beside another's: in one page, page after page of a warp, warp beside warp, block beside block."""
     g = torch.Generator().manual_seed(33)
@@ -64,6 +96,8 @@ def test_values_whose_exponents_lie_as_far_apart_as_they_can(cuda_device, monkey
     else:
         e = torch.randint(-95, 99, (n,), generator=g).float()
     kv[:, :, 1] *= torch.exp2(e.double())[:, None, None]
+    if how == "zeros":
+        kv[5::7, :, 1] = 0.0
     q = torch.randn((nh, hd), generator=g).to(torch.bfloat16)
     got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, blocks, 1.0 / math.sqrt(hd))
     _check(got, want, mag, n)
