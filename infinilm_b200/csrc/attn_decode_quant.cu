@@ -5,10 +5,11 @@
 //   s_k = scale q.K_k with K_k = c_k 2^e_k,  o = sum_k p_k V_k / sum_k p_k,  p_k = 2^(s_k log2 e - m),  V_k = d_k 2^f_k
 //
 // Codes become halves (exactly) in registers and go straight into m16n8k16 products with f32 sums; nothing is scaled before a
-// product. The exponent of K multiplies the score; the exponent of V joins the softmax's: with t_k = s_k log2 e + f_k and the running
-// maximum taken over t_k, the weight w_k = 2^(t_k - m) is what V's codes are multiplied by, at most 2^8 and therefore a half with 11 bits
-// where they count, and the denominator adds w_k 2^-f_k in 32 bits (2^-100 to 2^108 a key). Where exponents of V lie so far apart
-// that w_k may be 0 although p_k counts, the denominator's 2^(t_k - f_k - m) is an exponential of its own. A row of zeros counts as one of the lowest exponent. Else one a score, as without a quantised cache. q goes to halves times a
+// product. The exponent of K multiplies the score; the exponent of V joins the softmax's: with t_k = s_k log2 e + f_k and a reference m 7 below the
+// running maximum of t_k, the weight w_k = 2^(t_k - m) is what V's codes are multiplied by, at most 2^15 and therefore a half with 11 bits
+// where they count (down to 2^-21 of the largest; the smallest of a half is 2^-31 of it), and the denominator adds w_k 2^-f_k in 32 bits (2^-93 to 2^107 a key). Where exponents
+// of V lie so far apart that w_k may be 0 although p_k counts, the denominator's 2^(t_k - f_k - m) is an exponential of its own. A row of zeros counts as one of the lowest
+// exponent. Else one exponential a score, as without a quantised cache. q goes to halves times a
 // power of two of its row's (its largest magnitude then lies in 2^8 .. 2^9, so that a score times the largest power of two of K, 2^100, stays within 32 bits): what a half
 // cannot hold of it is below 2^-33 of that.
 //
@@ -62,8 +63,9 @@ __host__ __device__ constexpr int dq_smem(int rows) { return dq_q(rows) + rows *
 // 131,072, whole numbers, whose codes take more registers to convert, 22.1 / 24.8. Five spill: 29 to 30 for the last two.)
 constexpr int dq_per_sm(int kind, int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 2 && kind == KVQ_INT8 ? 3 : 4) : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
-constexpr float DQ_RAISE = 8.f;                   // the running maximum follows only when a page's is more than this above it (log2 units)
-// Bytes of V's exponents that are in order: 2^-80 .. 2^-1 (rows up to 224 in e4m3, 63 as whole numbers). Among these a weight that is flushed to 0, below 2^-126, has a score 2^46 below the best
+constexpr float DQ_RAISE = 8.f;                   // the reference follows the maximum only when a page's is more than this above it (log2 units)
+constexpr float DQ_UP = 7.f;                      // ... and lies this far below it: weights up to 2^15 (a half holds 65,504), so that small ones keep their bits down to 2^-21, and some down to 2^-31, of the largest
+// Bytes of V's exponents that are in order: 2^-80 .. 2^-1 (rows up to 224 in e4m3, 63 as whole numbers). Among these a weight that is flushed to 0, below 2^-126, has a score 2^53 below the best
 // one: no share of the denominator.
 constexpr unsigned DQ_V_LOW = 47, DQ_V_SPAN = 80;
 
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
                     }
                 }
             }
-            // how far above the maximum (which starts at the lowest float, so that no difference is one of infinities)
+            // how far above the reference (which starts at the lowest float, so that no difference is one of infinities)
             float dv[NT][4], top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
                     top = fmaxf(fmaxf(top, dv[j][2 * n]), dv[j][2 * n + 1]);
                 }
             }
-            if (__any_sync(0xffffffffu, top > DQ_RAISE || odd[0] || odd[1])) {           // also the first keys of a head
+            if (__any_sync(0xffffffffu, top > DQ_UP + DQ_RAISE || odd[0] || odd[1])) {           // also the first keys of a head
                 const bool far = __any_sync(0xffffffffu, odd[0] || odd[1]);
                 if (__builtin_expect(far, 0)) {
                     // A row of zeros has the exponent 2^0, far above its neighbours', and must not set the reference that their weights are rounded against: it gets the lowest.
@@ -437,7 +439,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
                         float mx = fmaxf(tv[j][i], tv[j][2 + i]);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                        const float mn = mx > m[j][i] + DQ_RAISE ? mx : m[j][i];
+                        const float mn = mx > m[j][i] + (far ? DQ_UP : DQ_UP + DQ_RAISE) ? mx - DQ_UP : m[j][i];     // (far: a key's share of the denominator stays below 2^107)
                         root[i] = dq_root(m[j][i], mn), corr[i] = root[i] * root[i];      // 0 when nothing was summed yet
                         m[j][i] = mn, dv[j][i] = tv[j][i] - mn, dv[j][2 + i] = tv[j][2 + i] - mn;
                     }

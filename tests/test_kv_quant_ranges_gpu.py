@@ -1,4 +1,5 @@
-"""Single tokens over the 8-bit cache where values differ most: rows of zeros with the highest scores, exponents as far apart as the format lets them be, keys and queries whose powers of two are far apart. Against 64 bits."""
+"""Single tokens over the 8-bit cache where values differ most: rows of zeros with the highest scores, exponents as far apart as the format lets them be, many small weights
+beside a large one, keys and queries whose powers of two are far apart. Against 64 bits."""
 import math
 
 import pytest
@@ -39,9 +40,9 @@ def _run(dev, monkeypatch, q, kv, kind, blocks, scale, order=None, window=None):
 
 
 def _check(got, want, mag, n):
-    # the output's rounding; weights as halves, 2^-11 each (below 2^-14 of the largest: 2^-25 of it a key, its row's largest code half of the largest there is); exponentials, exponents and
-    # sums in 32 bits: 2^-15 together
-    room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -24 * n * mag.amax(-1, keepdim=True)
+    # the output's rounding; weights as halves, 2^-11 each, and, where they are subnormal, by 2^-25 of a unit: the largest weight is 2^7 units at least, its row's largest code half
+    # of the largest there is, so 2^-31 of the largest column a key; exponentials, exponents and sums in 32 bits: 2^-15 together
+    room = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + mag * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -31 * n * mag.amax(-1, keepdim=True)
     off = (got - want).abs()
     assert (off <= room).all(), float((off / room.clamp(min=1e-300)).max())
 
@@ -100,6 +101,23 @@ def test_values_whose_exponents_lie_as_far_apart_as_they_can(cuda_device, monkey
         kv[5::7, :, 1] = 0.0
     q = torch.randn((nh, hd), generator=g).to(torch.bfloat16)
     got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, blocks, 1.0 / math.sqrt(hd))
+    _check(got, want, mag, n)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd", HEADS)
+@pytest.mark.parametrize("blocks", [0, 7, -8])
+def test_many_small_weights_beside_a_large_one(cuda_device, monkeypatch, kind, nh, nkv, hd, blocks):
+    """16,384 keys of 2^-26 of the largest weight each bring 2^-12 together, in a column of their own."""
+    g = torch.Generator().manual_seed(34)
+    n, u = 16385, _toward(hd, g)
+    kv = torch.zeros((n, nkv, 2, hd)).double()
+    kv[6000, :, 0] = 26 * math.log(2.0) * u
+    kv[:, :, 1, 1] = 1.0
+    kv[6000, :, 1, 1], kv[6000, :, 1, 0] = 0.0, 1.0
+    q = (math.sqrt(hd) * u).to(torch.bfloat16).expand(nh, hd).contiguous()
+    got, want, mag = _run(cuda_device, monkeypatch, q, kv, kind, blocks, 1.0 / math.sqrt(hd))
+    assert (want[:, 1] > 2.0 ** -13).all()
     _check(got, want, mag, n)
 
 
