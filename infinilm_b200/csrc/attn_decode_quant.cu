@@ -748,6 +748,7 @@ struct DqArgs {
     int kind, bt_stride, n_decode, nh, nkv, hd, window, n_blocks, early;
     float scale;
 };
+static_assert(sizeof(DqArgs) == 120, "what ops.py packs, padding included");
 IL_EXPORT int il_attn_decode_quant(const DqArgs* args) {
     const DqArgs& a = *args;
     const int kind = a.kind, n_decode = a.n_decode, nh = a.nh, nkv = a.nkv, hd = a.hd, n_blocks = a.n_blocks;

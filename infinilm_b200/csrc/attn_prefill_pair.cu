@@ -366,6 +366,7 @@ struct PpArgs {
     int bt_stride, first_entry, n_entries, n_tiles_total, nh, nkv, hd, window;
     float scale;
 };
+static_assert(sizeof(PpArgs) == 112, "what ops.py packs, padding included");
 IL_EXPORT int il_attn_prefill_pair(const PpArgs* args) {
     const auto [q, q_stride, out, kv_map, block_table, entry_qstart, entry_kvlen, status, stream, bt_stride, first_entry, n_entries, n_tiles_total, nh, nkv, hd, window, scale] = *args;
     if (n_tiles_total <= 0 || first_entry >= n_entries) return IL_OK;

@@ -219,6 +219,7 @@ struct KvqStoreArgs {
     int act_kind, bt_stride, kind, T, nh, nkv, hd, rot;
     float mscale;
 };
+static_assert(sizeof(KvqStoreArgs) == 120, "what ops.py packs, padding included");
 IL_EXPORT int il_rope_store_quant(const KvqStoreArgs* args) {
     const auto [qkv, row_stride, q_out, q_stride, tok_pos, tok_entry, block_table, cache, inv_freq, stream, act_kind, bt_stride, kind, T, nh, nkv, hd, rot, mscale] = *args;
     if (T <= 0) return IL_OK;
@@ -450,6 +451,7 @@ struct KvqUnpackArgs {
     int* status;
     int kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key, room;
 };
+static_assert(sizeof(KvqUnpackArgs) == 112, "what ops.py packs, padding included");
 IL_EXPORT int il_kv_unpack(const KvqUnpackArgs* args) {
     const auto [cache, block_table, entry_kvlen, entry_qstart, pages, table, stream, status, kind, bt_stride, window, first_entry, n_entries, width, nkv, hd, out_kind, told_by_key,
                 room] = *args;

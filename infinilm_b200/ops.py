@@ -1846,9 +1846,10 @@ def kv_quant_record(head_dim: int) -> int:
     return 2 * KV_QUANT_PAGE * head_dim + 2 * KV_QUANT_PAGE
 
 
-# Arguments of the entry points below as the structs that they take (a ctypes call with twenty arguments of its own costs 3 us of host time, between kernels of a few microseconds).
-_STORE_ARGS, _UNPACK_ARGS = struct.Struct("<QqQq6Q8if"), struct.Struct("<8Q11i")
-_DECODE_ARGS, _PAIR_ARGS = struct.Struct("<Qq8Q9if"), struct.Struct("<Qq7Q8if")
+# Arguments of the entry points below as the structs that they take (a ctypes call with twenty arguments of its own costs 3 us of host time, between kernels of a few microseconds). They are
+# copied whole there: the bytes that round a struct up to a multiple of eight belong to it.
+_STORE_ARGS, _UNPACK_ARGS = struct.Struct("<QqQq6Q8if4x"), struct.Struct("<8Q11i4x")
+_DECODE_ARGS, _PAIR_ARGS = struct.Struct("<Qq8Q9if"), struct.Struct("<Qq7Q8if4x")
 _quant_fns = {}
 
 

@@ -96,3 +96,20 @@ def test_head_sizes_without_kernels_over_codes_read_all_entries_back(monkeypatch
     calls = _step(monkeypatch, 4, 2, 48, dtype=dtype, portions=(5,))
     assert calls[0][0] == "kv_unpack" and calls[0][1]["first_entry"] == 0
     assert [c[0] for c in calls[1:]] == (["attention_plain"] if dtype is torch.float32 else ["attention_decode", "attention_prefill"])
+
+
+# ---- arguments ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("packed,file,name", [("_STORE_ARGS", "kv_quant.cu", "KvqStoreArgs"), ("_UNPACK_ARGS", "kv_quant.cu", "KvqUnpackArgs"),
+                                              ("_DECODE_ARGS", "attn_decode_quant.cu", "DqArgs"), ("_PAIR_ARGS", "attn_prefill_pair.cu", "PpArgs")])
+def test_packed_arguments_are_as_long_as_the_struct_that_is_read(packed, file, name):
+    """The entry points read a whole struct; its size stands in the source, where the compiler checks it, and follows from its members."""
+    text = _source(file)
+    size = int(re.search(r"static_assert\(sizeof\(%s\) == (\d+)," % name, text).group(1))
+    body = re.search(r"struct %s \{(.*?)\n\};" % name, text, re.S).group(1)
+    at, kind = 0, None
+    for member in (m for statement in body.split(";") if statement.strip() for m in statement.split(",")):
+        words = re.search(r"^\s*((?:const )?(?:void|float|int|long long|cudaStream_t))?\s*(\*?)\s*(\w+)\s*$", member)
+        kind = words.group(1) or kind
+        width = 8 if words.group(2) or kind in ("long long", "cudaStream_t") else 4
+        at = (at + width - 1) // width * width + width
+    assert (at + 7) // 8 * 8 == size == getattr(ops, packed).size
