@@ -1992,9 +1992,10 @@ def _quant_blocks(kind: int, head_dim: int, group: int, units: int, pages: int, 
     if most is None:
         fn = build.load("attn_decode_quant", {"HEAD_DIM": head_dim}).il_attn_decode_quant_resident_blocks
         fn.argtypes, fn.restype = [_c_int, _c_int], _c_int
-        most = _resident_quant[key] = int(fn(kind, group))
+        most = int(fn(kind, group))
         if most <= 0:
             raise KernelError("attention_decode_quant: the occupancy query failed")
+        _resident_quant[key] = most
     least, cluster = QUANT_LEAST_PAGES, 1
     if pages <= QUANT_WHOLE_PAGES:
         return 0

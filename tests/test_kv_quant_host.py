@@ -113,3 +113,14 @@ def test_packed_arguments_are_as_long_as_the_struct_that_is_read(packed, file, n
         width = 8 if words.group(2) or kind in ("long long", "cudaStream_t") else 4
         at = (at + width - 1) // width * width + width
     assert (at + 7) // 8 * 8 == size == getattr(ops, packed).size
+
+
+def test_an_occupancy_query_that_fails_is_asked_again(monkeypatch):
+    answers = [0, 592]
+    lib = SimpleNamespace(il_attn_decode_quant_resident_blocks=lambda kind, group: answers.pop(0))
+    monkeypatch.setattr(ops.build, "load", lambda *a: lib)
+    monkeypatch.setattr(ops, "_resident_quant", {})
+    with pytest.raises(ops.KernelError, match="occupancy"):
+        ops._quant_blocks(0, 128, 4, 64, 400, 0)
+    assert ops._quant_blocks(0, 128, 4, 64, 400, 0) == 592 and not answers
+    assert ops._quant_blocks(0, 128, 4, 64, 400, 0) == 592
