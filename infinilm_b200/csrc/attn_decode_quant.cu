@@ -195,12 +195,12 @@ __device__ __forceinline__ void dq_write(const float4& acc, float M, float L, __
         if (d == 0) *reinterpret_cast<float2*>(ml_part + 2 * r) = make_float2(M, L);
     }
 }
-// (q and the newest token's slot of the cache, and in the second kernel the parts, are written by the kernel before and read after a wait that is not the
-// kernel's first statement: they are not declared __restrict__.)
+// (q and the newest token's slot of the cache, without `early` also lengths and tables, and in the second kernel the parts, may be written by the kernel before and are then read after a wait:
+// they are not declared __restrict__, whose loads may be moved above it.)
 template <int KIND, int NT>
 __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decode_quant_kernel(
-    const __nv_bfloat16* q, long long q_stride, const unsigned char* cache, const int* __restrict__ block_table, int bt_stride,
-    const int* __restrict__ entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int per_unit, float* o_part, float* ml_part,
+    const __nv_bfloat16* q, long long q_stride, const unsigned char* cache, const int* block_table, int bt_stride,
+    const int* entry_kvlen, int n_decode, int nh, int nkv, int G, int row_tiles, float scale_log2, int window, int per_unit, float* o_part, float* ml_part,
     __nv_bfloat16* out, int* status, int early) {
     if (!early) il_pdl_wait();
     extern __shared__ __align__(128) unsigned char smem[];

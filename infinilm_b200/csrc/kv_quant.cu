@@ -6,6 +6,7 @@
 // may be the same place.
 // il_kv_unpack: pages of requests as pages of bfloat16 or float32 values in the layout of the plain cache, [page][K, V][kv head][16][head_dim].
 // Both are bound by memory: what they read and write is named at each kernel.
+// Positions, entries, tables and lengths may come from the kernel in front (no caller vouches that they do not), so they are not declared __restrict__: such loads may be moved above the wait.
 #include <algorithm>
 
 #include "kv_quant.cuh"
@@ -53,8 +54,8 @@ __device__ __forceinline__ uint2 kvq_codes8(const float (&x)[8], float f) {
 // 128, bfloat16, us: 230 with a column a lane at a time, 103 with a block a token and its angles in shared memory, 43 so, 40 with two columns rotated an instruction.
 constexpr int KVS_AHEAD = 1, KVS_WARPS = 148 * 16;
 template <typename TA, int KIND, int PER>
-__global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* __restrict__ tok_pos,
-                                                               const int* __restrict__ tok_entry, const int* __restrict__ block_table, int bt_stride,
+__global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* tok_pos,
+                                                               const int* tok_entry, const int* block_table, int bt_stride,
                                                                unsigned char* cache, int T, int nh, int nkv, int hd, int rot, const float* __restrict__ inv_freq, float mscale,
                                                                int wpt) {
     constexpr int HEADS = 32 / PER, OWN = 8 / HEADS > 0 ? 8 / HEADS : 1;      // heads of a round, angles that a lane makes
@@ -158,8 +159,8 @@ __global__ void __launch_bounds__(256, 4) rope_store_quant_kernel(const TA* qkv,
 
 // A warp a row (a head of q, k or v of one token), a lane the columns lane, lane + 32, ...: any even rot, any alignment.
 template <typename TA, int KIND>
-__global__ void __launch_bounds__(256) rope_store_quant_any_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* __restrict__ tok_pos,
-                                                                   const int* __restrict__ tok_entry, const int* __restrict__ block_table, int bt_stride,
+__global__ void __launch_bounds__(256) rope_store_quant_any_kernel(const TA* qkv, long long row_stride, TA* q_out, long long q_stride, const int* tok_pos,
+                                                                   const int* tok_entry, const int* block_table, int bt_stride,
                                                                    unsigned char* cache, int T, int nh, int nkv, int hd, int rot, const float* __restrict__ inv_freq, float mscale) {
     il_pdl_begin();
     const int rows = cache ? nh + 2 * nkv : nh, lane = threadIdx.x & 31, half = rot >> 1;
@@ -350,8 +351,8 @@ __device__ __forceinline__ void kvu_page(const unsigned char* recs, TO* out, int
 }
 
 template <typename TO, int KIND, int HD>
-__global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
-                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room, int* status) {
+__global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* cache, const int* block_table, int bt_stride, const int* entry_kvlen,
+                                                        const int* entry_qstart, int window, int first_entry, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room, int* status) {
     il_pdl_begin();
     const int hd = HD ? HD : hd_arg;
     const int i = blockIdx.y, e = first_entry + i, p = blockIdx.x;
@@ -383,8 +384,8 @@ __global__ void __launch_bounds__(256, 4) kv_unpack_kernel(const unsigned char* 
 
 // The same where tables are so wide, for so many requests, that most blocks of a page each might find nothing: the pages that are seen dealt out to KVU_BLOCKS blocks.
 template <typename TO, int KIND, int HD>
-__global__ void __launch_bounds__(256, 4) kv_unpack_dealt_kernel(const unsigned char* cache, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ entry_kvlen,
-                                                        const int* __restrict__ entry_qstart, int window, int first_entry, int n, int width, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room,
+__global__ void __launch_bounds__(256, 4) kv_unpack_dealt_kernel(const unsigned char* cache, const int* block_table, int bt_stride, const int* entry_kvlen,
+                                                        const int* entry_qstart, int window, int first_entry, int n, int width, int nkv, int hd_arg, TO* pages, int* table, int told_by_key, int room,
                                                         int* status) {
     il_pdl_begin();
     const int hd = HD ? HD : hd_arg;

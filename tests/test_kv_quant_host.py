@@ -124,3 +124,17 @@ def test_an_occupancy_query_that_fails_is_asked_again(monkeypatch):
         ops._quant_blocks(0, 128, 4, 64, 400, 0)
     assert ops._quant_blocks(0, 128, 4, 64, 400, 0) == 592 and not answers
     assert ops._quant_blocks(0, 128, 4, 64, 400, 0) == 592
+
+
+@pytest.mark.parametrize("file,kernels", [("kv_quant.cu", 4), ("attn_decode_quant.cu", 1)])
+def test_descriptors_that_the_kernel_in_front_may_write_are_not_declared_read_only(file, kernels):
+    """Nothing says that lengths, tables, positions and entries are older than the kernel in front of these calls (but `cached_before`): their kernels wait first and read them then. The kernel
+    that adds parts up stands behind one that has waited."""
+    found = 0
+    for kernel in re.split(r"__global__", _source(file))[1:]:
+        head = kernel.split("{", 1)[0]
+        if "merge_kernel" in head:
+            continue
+        found += 1
+        assert re.findall(r"__restrict__ (\w+)", head) in ([], ["inv_freq"]), head
+    assert found == kernels
