@@ -80,14 +80,21 @@ class Workspace:
         if buf is None or buf.numel() < n:
             if buf is not None:
                 self.version += 1
+                del buf, self._bufs[key]          # (first, so that both never exist together)
             buf = (torch.zeros if zero else torch.empty)(max(n, 1024), dtype=dtype, device=self.device)
             self._bufs[key] = buf
         return buf[:n]
 
     def address(self, tag: str, n: int, dtype: torch.dtype) -> int:
         """Where a `flat` buffer of at least n elements lies, for a kernel's argument."""
+        if self.size(tag, dtype) < n:
+            self.flat(tag, n, dtype)
+        return self._bufs[(tag, "flat", dtype)].data_ptr()
+
+    def size(self, tag: str, dtype: torch.dtype) -> int:
+        """Elements of a `flat` buffer as it stands; 0 where there is none yet."""
         buf = self._bufs.get((tag, "flat", dtype))
-        return buf.data_ptr() if buf is not None and buf.numel() >= n else self.flat(tag, n, dtype).data_ptr()
+        return 0 if buf is None else buf.numel()
 
     def whole(self, tag: str, dtype: torch.dtype) -> torch.Tensor:
         """All of a `flat` buffer as it stands; replaced when a request for more replaces it."""

@@ -2041,10 +2041,11 @@ def attention_decode_quant(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     group = n_heads // n_kv_heads
     n_blocks = _quant_blocks(k, head_dim, group, n_decode * n_kv_heads * (1 if group <= 8 else (group + 15) // 16), max(1, (seen + KV_QUANT_PAGE - 1) // KV_QUANT_PAGE), d)
     parts = n_blocks > 0
+    room = max(n_blocks, _resident_quant.get((d, k, head_dim, group > 8), 0))     # (one wave of blocks from the first call on: a workspace that grew makes captured steps stale)
     f = _quant_fns.get(("il_attn_decode_quant", head_dim)) or _quant_fn("il_attn_decode_quant", "attn_decode_quant", head_dim)
     _check(f(_packed(_DECODE_ARGS, what, q.data_ptr(), strides[0], out.data_ptr(), cache.data_ptr(), block_table.data_ptr(), entry_kvlen.data_ptr(),
-                               ws.address("quant_o_part", n_blocks * 32 * head_dim, torch.float32) if parts else 0,
-                               ws.address("quant_ml_part", n_blocks * 64, torch.float32) if parts else 0, _status_ptr(d), _raw_stream(d), k, table_shape[1], n_decode, n_heads,
+                               ws.address("quant_o_part", room * 32 * head_dim, torch.float32) if parts else 0,
+                               ws.address("quant_ml_part", room * 64, torch.float32) if parts else 0, _status_ptr(d), _raw_stream(d), k, table_shape[1], n_decode, n_heads,
                                n_kv_heads, head_dim, w, n_blocks, int(cached_before), scale)), what)
     if parts:
         count_launches(1)                         # the second kernel
@@ -2062,10 +2063,21 @@ def prefill_quant_tokens(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     return 2 * max(1, 128 // group) if head_dim <= 128 else max(1, prefill_tc5_rows(head_dim) // group)
 
 
+# Entries that only pad a step, at most (the engine's steps are rounded up by less).
+UNPACKED_SPARE = 128
+
+
 def unpacked_room(cache: torch.Tensor, n_entries: int, width: int) -> int:
     """Pages that reading back n_entries requests takes at most, packed: what their block tables can name, and no more than the cache has (a page belongs to one request; entries
-    that only pad a step have one page each)."""
-    return max(1, min(n_entries * width, cache.shape[0] + n_entries))
+    that only pad a step, up to UNPACKED_SPARE of them, have one page each)."""
+    return max(1, min(n_entries * width, cache.shape[0] + min(n_entries, UNPACKED_SPARE)))
+
+
+def hold_unpacked(ws, cache: torch.Tensor, n_entries: int, width: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype) -> None:
+    """Makes a workspace's room for pages read back, and their table, as large as any step over `cache` needs, so that no later step replaces it (which would make every captured step stale):
+    all of the cache's pages, and one for each entry that only pads a step."""
+    ws.address("kv_unpacked", (cache.shape[0] + UNPACKED_SPARE) * 2 * n_kv_heads * KV_QUANT_PAGE * head_dim, dtype)
+    ws.address("kv_unpacked_table", 1 << max(18, (n_entries * width - 1).bit_length()), torch.int32)      # (1 MB: 128 requests of 32,768 tokens; wider tables double it)
 
 
 def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype):
@@ -2078,6 +2090,9 @@ def unpacked_cache(ws, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torc
 def _unpacked_map(ws, n_pages: int, n_kv_heads: int, head_dim: int) -> Optional[torch.Tensor]:
     """The tensor map of a workspace's bfloat16 pages, of which there are n_pages at least; kept beside the buffer (one that grew is another one)."""
     per = 2 * n_kv_heads * KV_QUANT_PAGE * head_dim
+    if ws.size("kv_unpacked", torch.bfloat16) < n_pages * per:
+        for k in [k for k in ws.kept if k[0] == "kv_unpacked"]:
+            del ws.kept[k]                        # (else the buffer that is replaced would live on beside the new one)
     ws.address("kv_unpacked", n_pages * per, torch.bfloat16)
     whole, kept = ws.whole("kv_unpacked", torch.bfloat16), ws.kept.get(("kv_unpacked", n_kv_heads, head_dim))
     if kept is None or kept[0] is not whole:

@@ -97,11 +97,13 @@ class PagedAttend:
             return
         if fast and self.prefill_kernel != "mma" and ops.prefill_tc5_ok(self.hd, self.nh // self.nkv, cache.page_size):
             per = ops.prefill_quant_tokens(self.nh, self.nkv, self.hd)
+            ops.hold_unpacked(ctx.ws, cache.storage, E, width, self.nkv, self.hd, self.dtype)
             ops.attention_prefill_quant(qkv, out, cache.storage, cache.quant, cache.block_table, ctx.entry_qstart, ctx.entry_kvlen, n_dec, E, ctx.prompt_tiles(per),
                                         self.nh, self.nkv, self.hd, self.scale, self.mask_arg, ctx.ws, n_tiles_rule=(qkv.shape[0] - n_dec + per - 1) // per + E - n_dec - 1,
                                         room=ops.unpacked_room(cache.storage, E - n_dec, width))
             return
         first = n_dec if fast else 0
+        ops.hold_unpacked(ctx.ws, cache.storage, E, width, self.nkv, self.hd, self.dtype)
         pages, tma_map = ops.unpacked_cache(ctx.ws, ops.unpacked_room(cache.storage, E - first, width), self.nkv, self.hd, self.dtype)
         table = ctx.ws.flat("kv_unpacked_table", E * width, torch.int32).view(E, width)
         ops.kv_unpack(cache.storage, cache.quant, cache.block_table, ctx.entry_kvlen, pages, table, ctx.entry_qstart, self.mask_arg, first_entry=first, nan_in_keys=True, packed=True)

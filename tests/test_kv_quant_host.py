@@ -138,3 +138,69 @@ def test_descriptors_that_the_kernel_in_front_may_write_are_not_declared_read_on
         found += 1
         assert re.findall(r"__restrict__ (\w+)", head) in ([], ["inv_freq"]), head
     assert found == kernels
+
+
+# ---- workspaces ------------------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def launches(monkeypatch):
+    """The entry points with host tensors in place of the device's: everything up to the launch."""
+    monkeypatch.setattr(ops, "_on_one_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda d: 0)
+    monkeypatch.setattr(ops, "_status_ptr", lambda d: 0)
+    monkeypatch.setattr(ops, "_quant_fns", {})
+    monkeypatch.setattr(ops, "_quant_fn", lambda *a: (lambda args: 0))
+    monkeypatch.setattr(ops, "_prefill_tc5_fn", lambda hd: (lambda *a: 0))
+    monkeypatch.setattr(ops, "kv_tensor_map", lambda t: torch.zeros(ops.KV_MAP_BYTES, dtype=torch.uint8))
+    monkeypatch.setattr(ops, "_has_third_map", lambda m: True)
+    monkeypatch.setattr(ops, "attention_plain", lambda *a: None)
+    monkeypatch.setattr(ops, "_resident_quant", {(0, 1, 64, wide): 592 for wide in (False, True)})
+
+
+@pytest.mark.parametrize("dtype,nh", [(torch.bfloat16, 4), (torch.bfloat16, 132), (torch.float32, 4)])
+def test_later_steps_leave_the_workspace_as_the_first_made_it(launches, dtype, nh):
+    """Chunks of a growing prompt, more requests, wider tables: a buffer that was replaced would make every captured step stale."""
+    nkv, hd, pages = (2 if nh < 9 else 1), 64, 300
+    core = PagedAttend(dtype, nh, nkv, hd, 0.1)
+    storage, ws, seen = torch.zeros((pages, nkv, ops.kv_quant_record(hd)), dtype=torch.uint8), Workspace("cpu", 512), []
+    for lengths, portions, width in ([[5], [5], 1], [[80, 40], [75, 1], 5], [[2000, 300], [1000, 1], 125], [[4000] + [1] * 140, [64] + [1] * 140, 256], [[300] * 16, [1] * 16, 20]):
+        order = sorted(range(len(portions)), key=lambda i: portions[i] != 1)
+        kvlen, qlen = [lengths[i] for i in order], [portions[i] for i in order]
+        n_dec, E, T = sum(q == 1 for q in qlen), len(qlen), sum(qlen)
+        ctx = SimpleNamespace(n_decode=n_dec, n_entries=E, ws=ws, h_kvlen=kvlen, entry_kvlen=torch.tensor(kvlen, dtype=torch.int32), tok_pos=torch.zeros(T, dtype=torch.int32),
+                              entry_qstart=torch.zeros(E + 1, dtype=torch.int32), tok_entry=torch.zeros(T, dtype=torch.int32), prompt_tiles=lambda n: sum((q + n - 1) // n for q in qlen[n_dec:]))
+        core.run(torch.zeros((T, nh * hd), dtype=dtype), torch.zeros((T, nh * hd), dtype=dtype), ctx,
+                 PagedKVView(storage, torch.zeros((E, width), dtype=torch.int32), 16, max_pages=width, quant="int8"))
+        seen.append(ws.version)
+    assert seen == [seen[0]] * len(seen), seen
+
+
+def test_parts_have_room_for_a_wave_of_blocks_from_the_first_call_on(launches):
+    nh, nkv, hd, ws, seen = 8, 2, 64, Workspace("cpu", 64), []
+    cache = torch.zeros((2, nkv, ops.kv_quant_record(hd)), dtype=torch.uint8)
+    for n, length in ((1, 4000), (2, 9000), (8, 30000), (8, 131072)):
+        q = torch.zeros((n, nh * hd), dtype=torch.bfloat16)
+        ops.attention_decode_quant(q, q.clone(), cache, "int8", torch.zeros((n, 2), dtype=torch.int32), torch.zeros(n, dtype=torch.int32), n, nh, nkv, hd, 0.1, None, length, ws)
+        seen.append((ws.version, ws.size("quant_o_part", torch.float32)))
+    assert seen == [(0, 592 * 32 * hd)] * 4, seen
+
+
+def test_a_workspace_that_grows_does_not_keep_what_it_replaces(launches):
+    import gc
+    import weakref
+    ws = Workspace("cpu", 64)
+    ops._unpacked_map(ws, 10, 2, 64)
+    old = weakref.ref(ws.whole("kv_unpacked", torch.bfloat16))
+    gc.collect()
+    alive = []
+    real = torch.empty
+    try:
+        torch.empty = lambda *a, **kw: (alive.append(old() is not None), real(*a, **kw))[1]
+        ops._unpacked_map(ws, 500, 2, 64)
+    finally:
+        torch.empty = real
+    assert alive == [False] and ws.version == 1
+
+
+def test_steps_are_padded_by_fewer_entries_than_room_is_held_for():
+    from infinilm_b200.engine.step import _ENTRY_BUCKETS, _bucket
+    assert max(_bucket(n, _ENTRY_BUCKETS) - n for n in range(1, 5000)) < ops.UNPACKED_SPARE

@@ -51,3 +51,27 @@ def test_single_tokens_beside_portions(cuda_device, kind, nh, nkv, hd, prefill, 
             assert ((got[t].double().view(nh, hd) - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -7) * want.abs() + (2.0 ** -8 + 2.0 ** -14) * mag).all(), (e, i)
             t += 1
     ops.check_status("cuda:0")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_growing_prompt_leaves_captured_steps_as_they_are(cuda_device, dtype):
+    """Decode steps are captured, then a long prompt comes in chunks beside them and after it more requests: the same graphs are replayed on."""
+    from infinilm_b200.engine import StepEntry
+    from test_kv_quant_engine_gpu import _config, _engine
+    from tiny_configs import make_weights, random_ids
+    eng = _engine(_config(64, dtype), make_weights(_config(64, dtype), 6), dtype, "int8")
+    eng.enable_graphs()
+    a, b = eng.open("a"), eng.open("b")
+    eng.step([StepEntry(a, random_ids(20, 320, 1), [19])])
+    for t in range(4):
+        eng.step([StepEntry(a, [t], [0])])
+    version, graphs = eng.runner.ws.version, {k: g.graph for k, g in eng.runner._graphs.items() if g.graph is not None}
+    assert len(graphs) == 1
+    for chunk in (17, 64, 130, 150):
+        eng.step([StepEntry(b, random_ids(chunk, 320, chunk), [chunk - 1])])
+        eng.step([StepEntry(a, [3], [0])])
+    for i in range(5):
+        c = eng.open(("c", i))
+        eng.step([StepEntry(a, [5], [0]), StepEntry(c, random_ids(30 + i, 320, i), [0])])
+    eng.synchronize()
+    assert eng.runner.ws.version == version and all(eng.runner._graphs[k].graph is g for k, g in graphs.items())
