@@ -56,6 +56,10 @@ class Engine:
                                   device=self.device, dtype=self.dtype)
         self.runner = StepRunner(self.model, self.cache, self.device, max_batch_tokens)
         self.runner.max_positions = config.max_position_embeddings
+        for grp in self.cache.groups:             # room for prompts over 8-bit codes: what does not fit fails here and not in the middle of serving
+            if grp.need.quant is not None:
+                for storage in grp.storage.values():
+                    ops.hold_unpacked(self.runner.ws, storage, max_seqs, 1, grp.need.n_kv_heads, grp.need.head_dim, self.dtype)
         self.vocab_size = self.model.vocab
 
     # -- construction ----------------------------------------------------------------------

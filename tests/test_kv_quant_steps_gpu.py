@@ -56,10 +56,13 @@ def test_single_tokens_beside_portions(cuda_device, kind, nh, nkv, hd, prefill, 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_a_growing_prompt_leaves_captured_steps_as_they_are(cuda_device, dtype):
     """Decode steps are captured, then a long prompt comes in chunks beside them and after it more requests: the same graphs are replayed on."""
+    from infinilm_b200 import ops
     from infinilm_b200.engine import StepEntry
     from test_kv_quant_engine_gpu import _config, _engine
     from tiny_configs import make_weights, random_ids
     eng = _engine(_config(64, dtype), make_weights(_config(64, dtype), 6), dtype, "int8")
+    ws, room = eng.runner.ws, (eng.cache.groups[0].storage[0].shape[0] + ops.UNPACKED_SPARE) * 2 * 2 * 16 * 64
+    assert ws.size("kv_unpacked", eng.dtype) == room          # held before the first request
     eng.enable_graphs()
     a, b = eng.open("a"), eng.open("b")
     eng.step([StepEntry(a, random_ids(20, 320, 1), [19])])
