@@ -89,7 +89,7 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
-    takes_quant_cache = False                     # True: the parameter `kv_cache` (a kind of 8-bit codes) makes its cache one of codes
+    takes_quant_cache = False                     # True: the parameter `kv_cache` (a kind of 8-bit codes) makes its cache one of codes (softmax of scaled scores only: no sink, bias, cap or sigmoid)
 
     def cache_need(self):
         """None, one `CacheNeed`, or a tuple of them (pages and a state, two states): `forward` then gets None, one cache
