@@ -24,7 +24,7 @@
 //   (warp w takes pages w, w + 4, ... of it; a page's record of a kv head is one untiled bulk copy into the warp's own ring) and merged
 //   in shared memory. A unit that lies in one block is final there, else its parts go to scratch. Short requests: a block a unit, all of them final
 //   (per_unit 1). In between, where one wave of blocks holds two to eight blocks a unit that are not much longer than dealt out: a cluster of them (per_unit), whose blocks read each other's parts
-//   from shared memory: no scratch, no second kernel (eight requests of 1,024 tokens, 32 heads on 8 of 128, 10.2 -> 8.1 us).
+//   from shared memory: no scratch, no second kernel (eight requests of 1,024 tokens, 32 heads on 8 of 128, 10.0 -> 8.4 us).
 //   (Parts added up by the block that finishes last, with fences and counts, took 8 us more than blocks that are final; the second kernel takes 2 to 3.)
 //
 // Token t (= entry t) sits at position kvlen - 1 and sees positions max(0, kvlen - window) .. kvlen - 1 (window < 0: runs of -window; 0: all). No
@@ -41,14 +41,14 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128 || HEAD_DIM == 256, "the 8-bit d
 
 constexpr int DQ_HD = HEAD_DIM;
 constexpr int DQ_REC = kvq_record(HEAD_DIM);
-constexpr int DQ_STAGES = 2;                      // records of a warp's ring: three gain nothing (105, 111 us for 64 requests of up to 8,192 tokens, 32 heads on 8 of 128)
+constexpr int DQ_STAGES = 2;                      // records of a warp's ring: three gain nothing (105, 111 us when tried, 64 requests of up to 8,192 tokens, 32 heads on 8 of 128)
 constexpr int DQ_CH = HEAD_DIM / 16;               // pieces of 16 columns of a head
 constexpr int DQ_KG = HEAD_DIM / 64;              // groups of four product steps of Q.K^T
 constexpr int DQ_MT = HEAD_DIM / 16;              // tiles of 16 columns of V
 constexpr int DQ_VB = HEAD_DIM / 8 < 16 ? HEAD_DIM / 8 : 16;      // columns a lane takes of a key row at a time
 constexpr int DQ_NVB = HEAD_DIM / 8 / DQ_VB;      // ... and how often
 constexpr int DQ_WARPS = 4;
-// Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 11.0 / 9.7 (fewer parts to add up); one of 512 7.4 / 7.9, of 8,192 9.4 / 8.2.
+// Pages of a block at least. Four and eight, us: eight requests of 2,048 tokens, 32 heads on 2 of 128, 11.3 / 10.4 (fewer parts to add up); one of 512 8.0 / 8.2, of 8,192 9.9 / 9.2.
 constexpr int DQ_LEAST = 8;
 constexpr int DQ_OS = HEAD_DIM + 4;
 constexpr int DQ_CLUSTER = 8;                    // blocks of a cluster at most
@@ -59,14 +59,17 @@ __host__ __device__ constexpr int dq_bars(int rows) {
 }
 __host__ __device__ constexpr int dq_q(int rows) { return dq_bars(rows) + (DQ_WARPS * DQ_STAGES * 8 + 15) / 16 * 16; }          // q's halves and the heads' factors
 __host__ __device__ constexpr int dq_smem(int rows) { return dq_q(rows) + rows * DQ_HD * 2 + rows * 4; }
-// Blocks an SM that the registers are to allow. (Heads of 128, three / four, us: 64 requests of up to 8,192 tokens, 32 heads on 8, e4m3, 107.5 / 106.0; 32 of 4,096, 32 on 2, e4m3, 20.8 / 19.4; one of
-// 131,072, whole numbers, whose codes take more registers to convert, 22.1 / 24.8. Five spill: 29 to 30 for the last two.)
+// Blocks an SM that the registers are to allow. (Heads of 128, three / four, us: 64 requests of up to 8,192 tokens, 32 heads on 8, e4m3, 107.6 / 105.9; 32 of 4,096, 32 on 2, e4m3, 21.5 / 20.2; one of
+// 131,072 in e4m3 20.9 / 22.5, in whole numbers, whose codes take more registers to convert, 22.7 / 24.7. With four, the form for e4m3 with two column tiles spills 32 bytes a thread, heads of 256 up to 20;
+// five spill more: 29 to 30 us for the last two.)
 constexpr int dq_per_sm(int kind, int nt) { return HEAD_DIM == 64 ? (nt == 1 ? 5 : 4) : HEAD_DIM == 128 ? (nt == 2 && kind == KVQ_INT8 ? 3 : 4) : (nt == 1 ? 3 : 2); }
 constexpr unsigned DQ_SPIN = 1u << 24;
 constexpr float DQ_RAISE = 8.f;                   // the reference follows the maximum only when a page's is more than this above it (log2 units)
 constexpr float DQ_UP = 7.f;                      // ... and lies this far below it: weights up to 2^15 (a half holds 65,504), so that small ones keep their bits down to 2^-21, and some down to 2^-31, of the largest
 // Bytes of V's exponents that are in order: 2^-80 .. 2^-1 (rows up to 224 in e4m3, 63 as whole numbers). Among these a weight that is flushed to 0, below 2^-126, has a score 2^53 below the best
 // one: no share of the denominator.
+// Rows beyond (32 requests of 4,096, 32 heads on 2 of 128, e4m3, us: 18.6 in order, 24.1 where V is in the thousands; 64 of 4,500, 32 on 8, 99.7 / 104) and of zeros (25.2 / 109 with one on
+// each page) take the long way.
 constexpr unsigned DQ_V_LOW = 47, DQ_V_SPAN = 80;
 
 __device__ __forceinline__ void dq_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -324,7 +327,7 @@ __global__ void __launch_bounds__(DQ_WARPS * 32, dq_per_sm(KIND, NT)) attn_decod
         il_f2 l[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) m[j][0] = m[j][1] = -FLT_MAX, l[j] = il_f2_dup(0.f);
-        unsigned v_low = DQ_V_LOW;
+        unsigned v_low = DQ_V_LOW;                // (256: none is in order any more)
         for (int it = 0; it < n_my; ++it) {
             if (!dq_wait(bars + (done + it) % DQ_STAGES * 8, (done + it) / DQ_STAGES & 1)) {
                 if (lane == 0) atomicExch(status, 91);

@@ -1978,9 +1978,9 @@ _resident_quant = {}
 # How a unit's pages meet blocks. A block a unit, with every sum final, where dealing the pages out to one wave of blocks would take less than so many off the longest block: the second
 # kernel then costs more than it saves. Else a cluster of two to eight blocks a unit, which add their parts up themselves, while that leaves a block few enough more than dealing out does
 # (fewer with two column tiles of heads, where a page takes longer) and no more than QUANT_CLUSTER_MOST. All units count as long as the longest here, which a batch
-# of one long request among short ones would pay for: hence also QUANT_WHOLE_MOST (74 requests of 2,048, 32 on 8, 51.0 whole, 53.1 dealt out; of 4,096, heads of 64, 63.6 / 63.3). Whole / cluster / dealt out, us, heads
-# of 128: 64 requests of 256 tokens (16 pages), 32 heads on 8, 9.0 / - / 14.9; one of 256, 32 on 2, 6.7 / 6.6 / 7.4; of 512 9.3 / 6.7 / 7.8; of 1,536 - / 8.4 / 8.7; of 2,048 - / 9.3 / 8.7; three of 100, eight heads of 64, 4.3 / 5.1 / 8.9; eight
-# of 1,024, 32 on 8, - / 8.1 / 10.2; four of 2,560 - / 9.3 / 12.2; sixteen of 1,024 15.5 / 12.0 / 15.1; one of 4,096 - / 9.3 / 8.1.
+# of one long request among short ones would pay for: hence also QUANT_WHOLE_MOST (74 requests of 2,048, 32 on 8, 50.6 whole, 52.9 dealt out). Whole / cluster / dealt out, us, e4m3, heads
+# of 128: 64 requests of 256 tokens (16 pages), 32 heads on 8, 8.8 / 15.0 / 14.9; one of 256, 32 on 2, 7.9 / 6.8 / 8.3; of 512 10.8 / 6.9 / 8.3; of 1,536 23 / 8.5 / 8.8; of 2,048 30 / 9.4 / 8.8; three of 100, eight heads of 64, 4.3 / 5.1 / 9.0;
+# eight of 1,024, 32 on 8, 11.9 / 8.4 / 10.0; four of 2,560 24 / 9.6 / 12.2; sixteen of 1,024 12.0 / 10.4 / 13.4; one of 4,096 55 / 12.5 / 9.3.
 QUANT_LEAST_PAGES, QUANT_WHOLE_PAGES, QUANT_WHOLE_MOST, QUANT_CLUSTER_PAGES, QUANT_CLUSTER_MOST = 8, 12, 128, (12, 6), 32
 
 

@@ -85,8 +85,8 @@ class PagedAttend:
         return max(1, min(target // base, (max_pages + 3) // 4, 128))
 
     def run_quant(self, qkv, out, ctx, cache) -> None:
-        """The same over a cache of 8-bit codes, for plain scores (the mixers that take such a cache have no sink, bias, cap or sigmoid): its own kernels where the compute dtype and the head size have them, else the pages are read back and attended over as a plain cache's
-        (for the rows that no kernel over codes has been through)."""
+        """The same over a cache of 8-bit codes, for plain scores (the mixers that take such a cache have no sink, bias, cap or sigmoid): its own kernels where the
+        compute dtype and the head size have them, else the pages are read back and attended over as a plain cache's (for the rows that no kernel over codes has been through)."""
         n_dec, E, width = ctx.n_decode, ctx.n_entries, cache.block_table.shape[1]
         fast = self.dtype == torch.bfloat16 and not self.force_plain and self.hd in ops.QUANT_HEAD_DIMS
         if fast and n_dec > 0:
